@@ -34,6 +34,43 @@ int ce_loss(const float* gmax, const float* sumexp, const float* selected, int M
             float* mean_loss, float scale, cudaStream_t s);
 int ce_bwd(void* logits, int64_t ld, int M, int V, const int64_t* targets, int64_t start,
            const float* gmax, const float* sumexp, float scale, const float* scale_ptr, cudaStream_t s);
+// Storage types of the row kernels below.
+constexpr int kTypeBF16 = 0, kTypeFP16 = 1, kTypeFP32 = 2;
+// Scores of given tokens (score.cu).  `record` (or null): the rank's partial result
+// [rows][4 + 2k] instead of the final one.  state is [3][rows].
+int score_fwd(const void* logits, int type, int64_t ld, int64_t rows, int64_t vocab, const int64_t* targets,
+              int64_t start, int64_t vocab_total, int k, float* logprob, float* entropy, float* state,
+              float* top_value, int64_t* top_id, float* record, cudaStream_t s);
+int score_merge(const float* records, int parts, int64_t rows, int64_t vocab, const int64_t* targets, int k,
+                float* logprob, float* entropy, float* state, float* top_value, int64_t* top_id, cudaStream_t s);
+int score_bwd(const void* logits, int type, int64_t ld, int64_t rows, int64_t vocab, const int64_t* targets,
+              int64_t start, int64_t vocab_total, const float* state, const float* dlogprob, const float* dentropy,
+              void* out, int64_t ld_out, cudaStream_t s);
+// Activations in 8 bits (actpack.cu): BF16 or FP32 values
+int64_t act_pack_row_bytes(int64_t cols);
+int act_pack(const void* x, int type, int64_t ld, void* data, int64_t rows, int64_t cols, cudaStream_t s);
+int act_unpack(const void* data, void* out, void* act, int type, int64_t rows, int64_t cols, cudaStream_t s);
+// Block joint (join.cu): BF16 or FP32 values
+constexpr int64_t kJoinMaxCols = 8192;  // sixteen columns a thread, 512 threads
+int64_t join_max_cols();
+int join_bwd_parts(int64_t rows, int64_t cols);  // CTAs, each with its own column sums
+int join_fwd(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int type, const void* pw, const void* pb,
+             const void* gate, const void* w, const void* b, void* u, void* h, int64_t ld_h, float* stats, int64_t rows,
+             int64_t cols, float alpha, float eps, cudaStream_t s);
+struct JoinBwdCall {
+  const void *dh, *du, *u, *y;  // du may be null; y null: no branch (LayerNorm alone)
+  int64_t ld_dh, ld_du, ld_u, ld_y;
+  const void *pw, *pb, *gate, *w, *b;
+  const float *mean_y, *rstd_y, *mean_u, *rstd_u;  // *_y unused without a branch
+  void *dx, *dy, *h;  // h may be null
+  int64_t ld_dx, ld_dy;
+  void *dpw, *dpb, *dgate, *dw, *db;
+  float* workspace;  // join_bwd_parts * (4, or 2 without a branch) * cols
+  int64_t rows, cols;
+  int type, packed;
+  float alpha;
+};
+int join_bwd(const JoinBwdCall& call, cudaStream_t s);
 // Optimizer (optim.cu)
 int grad_sqsum_parts(int64_t n);
 int grad_sqsum(const void* grad, int is_fp32, int64_t n, double* partial, double* out, int accumulate,

@@ -206,6 +206,211 @@ void attention_bwd_tc(const at::Tensor& qkv, const at::Tensor& out, const at::Te
                          dbg_words(dbg, 1, B * H * (S / 128))),
      "attention_bwd_tc");
 }
+
+// Numbers go into messages as text: c10's message stream crashes on integers where
+// the extension and libtorch were linked against different C++ runtimes.
+std::string shape_text(int64_t rows, int64_t cols) {
+  return "[" + std::to_string(rows) + ", " + std::to_string(cols) + "]";
+}
+// Row kernels: storage type code, and the checks shared by their bindings.
+int type_code(const at::Tensor& t, bool half, const char* name) {
+  if (t.scalar_type() == at::kBFloat16) return k::kTypeBF16;
+  if (t.scalar_type() == at::kFloat) return k::kTypeFP32;
+  TORCH_CHECK(half && t.scalar_type() == at::kHalf, name, " has the wrong dtype");
+  return k::kTypeFP16;
+}
+void need_like(const at::Tensor& t, const at::Tensor& like, at::ScalarType dt, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == dt, name, " has the wrong dtype");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+void need_rows(const at::Tensor& t, const at::Tensor& like, int64_t rows, int64_t cols, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has the wrong dtype");
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && (t.stride(1) == 1 || cols == 1), name,
+              " must be ", shape_text(rows, cols), " with contiguous rows");
+}
+void need_vector(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
+  need_like(t, like, like.scalar_type(), name);
+  TORCH_CHECK(t.numel() == n, name, " must hold ", std::to_string(n), " values");
+}
+void need_floats(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
+  need_like(t, like, at::kFloat, name);
+  TORCH_CHECK(t.numel() >= n, name, " must hold ", std::to_string(n), " values");
+}
+
+void score_fwd(const at::Tensor& logits, const at::Tensor& targets, int64_t start, int64_t vocab_total, int64_t top_k,
+               const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& top_ids,
+               const c10::optional<at::Tensor>& record) {
+  // out: FP32 [5 + top_k rows' worth]: logprob, entropy, state[3], then the alternatives' log probabilities.
+  const int type = type_code(logits, true, "logits");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  need_rows(logits, logits, rows, vocab, "logits");
+  need_like(targets, logits, at::kLong, "targets");
+  TORCH_CHECK(targets.numel() == rows, "targets must hold one id a row");
+  float* f = nullptr;
+  int64_t* ids = nullptr;
+  float* rec = nullptr;
+  if (record) {
+    need_floats(*record, logits, rows * (4 + 2 * top_k), "record");
+    rec = record->data_ptr<float>();
+  } else {
+    TORCH_CHECK(out && (top_ids || !top_k), "out and top_ids are needed without a record");
+    need_floats(*out, logits, rows * (5 + top_k), "out");
+    f = out->data_ptr<float>();
+    if (top_k) {
+      need_like(*top_ids, logits, at::kLong, "top_ids");
+      TORCH_CHECK(top_ids->numel() == rows * top_k, "top_ids must hold top_k ids a row");
+      ids = top_ids->data_ptr<int64_t>();
+    }
+  }
+  const c10::cuda::CUDAGuard g(logits.device());
+  ok(k::score_fwd(logits.data_ptr(), type, logits.stride(0), rows, vocab, targets.data_ptr<int64_t>(), start,
+                  vocab_total, int(top_k), f, f + rows, f + 2 * rows, f + 5 * rows, ids, rec, cur()), "score_fwd");
+}
+void score_merge(const at::Tensor& records, const at::Tensor& targets, int64_t vocab, int64_t top_k, at::Tensor& out,
+                 at::Tensor& top_ids) {
+  const int64_t rows = targets.numel(), parts = records.size(0);
+  need_like(targets, records, at::kLong, "targets");
+  need_floats(records, records, parts * rows * (4 + 2 * top_k), "records");
+  need_floats(out, records, rows * (5 + top_k), "out");
+  need_like(top_ids, records, at::kLong, "top_ids");
+  TORCH_CHECK(records.is_cuda() && top_ids.numel() == rows * top_k, "top_ids must hold top_k ids a row");
+  float* f = out.data_ptr<float>();
+  const c10::cuda::CUDAGuard g(records.device());
+  ok(k::score_merge(records.data_ptr<float>(), int(parts), rows, vocab, targets.data_ptr<int64_t>(), int(top_k), f,
+                    f + rows, f + 2 * rows, f + 5 * rows, top_ids.data_ptr<int64_t>(), cur()), "score_merge");
+}
+void score_bwd(const at::Tensor& logits, const at::Tensor& targets, int64_t start, int64_t vocab_total,
+               const at::Tensor& state, const at::Tensor& dlogprob, const c10::optional<at::Tensor>& dentropy,
+               at::Tensor& out) {
+  const int type = type_code(logits, true, "logits");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  need_rows(logits, logits, rows, vocab, "logits");
+  need_rows(out, logits, rows, vocab, "out");
+  need_like(targets, logits, at::kLong, "targets");
+  TORCH_CHECK(targets.numel() == rows, "targets must hold one id a row");
+  need_floats(state, logits, 3 * rows, "state");
+  need_floats(dlogprob, logits, rows, "dlogprob");
+  if (dentropy) need_floats(*dentropy, logits, rows, "dentropy");
+  const c10::cuda::CUDAGuard g(logits.device());
+  ok(k::score_bwd(logits.data_ptr(), type, logits.stride(0), rows, vocab, targets.data_ptr<int64_t>(), start,
+                  vocab_total, state.data_ptr<float>(), dlogprob.data_ptr<float>(),
+                  dentropy ? dentropy->data_ptr<float>() : nullptr, out.data_ptr(), out.stride(0), cur()),
+     "score_bwd");
+}
+
+void need_packed(const at::Tensor& data, const at::Tensor& like, int64_t rows, int64_t cols, const char* name) {
+  TORCH_CHECK(data.is_cuda() && data.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(data.scalar_type() == at::kByte && data.dim() == 2 && data.is_contiguous() && data.size(0) == rows &&
+                  data.size(1) == k::act_pack_row_bytes(cols),
+              name, " is not the packed form of ", shape_text(rows, cols));
+}
+void act_pack(const at::Tensor& x, at::Tensor& data) {
+  const int type = type_code(x, false, "x");
+  need_rows(x, x, x.size(0), x.size(1), "x");
+  need_packed(data, x, x.size(0), x.size(1), "data");
+  const c10::cuda::CUDAGuard g(x.device());
+  ok(k::act_pack(x.data_ptr(), type, x.stride(0), data.data_ptr(), x.size(0), x.size(1), cur()), "act_pack");
+}
+void act_unpack(const at::Tensor& data, at::Tensor& out, const c10::optional<at::Tensor>& act) {
+  const int type = type_code(out, false, "out");
+  const int64_t rows = out.size(0), cols = out.size(1);
+  need_like(out, data, out.scalar_type(), "out");
+  need_packed(data, out, rows, cols, "data");
+  if (act) {
+    need_like(*act, out, out.scalar_type(), "act");
+    TORCH_CHECK(act->sizes() == out.sizes(), "act and out differ in shape");
+  }
+  const c10::cuda::CUDAGuard g(out.device());
+  ok(k::act_unpack(data.data_ptr(), out.data_ptr(), act ? act->data_ptr() : nullptr, type, rows, cols, cur()),
+     "act_unpack");
+}
+
+void join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tensor& pw, const at::Tensor& pb,
+              const at::Tensor& gate, const at::Tensor& w, const at::Tensor& b, at::Tensor& u, at::Tensor& h,
+              at::Tensor& stats, double alpha, double eps) {
+  const int type = type_code(x, false, "x");
+  const int64_t rows = x.size(0), cols = x.size(1);
+  need_rows(x, x, rows, cols, "x"); need_rows(y, x, rows, cols, "y");
+  need_rows(h, x, rows, cols, "h"); need_rows(u, x, rows, cols, "x_out");
+  TORCH_CHECK(u.is_contiguous(), "x_out must be contiguous");
+  need_vector(pw, x, cols, "post_weight"); need_vector(pb, x, cols, "post_bias"); need_vector(gate, x, cols, "gate");
+  need_vector(w, x, cols, "pre_weight"); need_vector(b, x, cols, "pre_bias");
+  need_floats(stats, x, 4 * rows, "stats");
+  const c10::cuda::CUDAGuard g(x.device());
+  ok(k::join_fwd(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), type, pw.data_ptr(), pb.data_ptr(),
+                 gate.data_ptr(), w.data_ptr(), b.data_ptr(), u.data_ptr(), h.data_ptr(), h.stride(0),
+                 stats.data_ptr<float>(), rows, cols, float(alpha), float(eps), cur()), "block_join_fwd");
+}
+int64_t join_bwd_workspace(int64_t rows, int64_t cols, bool branch) {
+  return k::join_bwd_parts(rows, cols) * (branch ? 4 : 2) * cols;
+}
+// Gradients of the joint, or of LayerNorm alone where `y` is absent.  `u` and `y` are
+// both packed (bytes) or both of dh's type.  grads: dpre_weight, dpre_bias and, with a
+// branch, dpost_weight, dpost_bias, dgate, [2 or 5, cols].
+void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const at::Tensor& u,
+              const c10::optional<at::Tensor>& y, const at::Tensor& mean_u, const at::Tensor& rstd_u,
+              const c10::optional<at::Tensor>& mean_y, const c10::optional<at::Tensor>& rstd_y,
+              const c10::optional<at::Tensor>& pw, const c10::optional<at::Tensor>& pb,
+              const c10::optional<at::Tensor>& gate, const at::Tensor& w, const c10::optional<at::Tensor>& b,
+              at::Tensor& dx, const c10::optional<at::Tensor>& dy, const c10::optional<at::Tensor>& h,
+              at::Tensor& grads, at::Tensor& workspace, double alpha) {
+  k::JoinBwdCall c = {};
+  c.type = type_code(dh, false, "dh");
+  const int64_t rows = dh.size(0), cols = dh.size(1);
+  c.rows = rows;
+  c.cols = cols;
+  c.packed = u.scalar_type() == at::kByte;
+  c.alpha = float(alpha);
+  need_rows(dh, dh, rows, cols, "dh"); need_rows(dx, dh, rows, cols, "dx");
+  auto kept = [&](const at::Tensor& t, const char* name) {
+    if (c.packed) need_packed(t, dh, rows, cols, name);
+    else need_rows(t, dh, rows, cols, name);
+  };
+  kept(u, "x_out");
+  need_floats(mean_u, dh, rows, "mean"); need_floats(rstd_u, dh, rows, "rstd");
+  need_vector(w, dh, cols, "pre_weight");
+  c.dh = dh.data_ptr(); c.ld_dh = dh.stride(0);
+  c.dx = dx.data_ptr(); c.ld_dx = dx.stride(0);
+  c.u = u.data_ptr(); c.ld_u = u.stride(0);
+  c.mean_u = mean_u.data_ptr<float>(); c.rstd_u = rstd_u.data_ptr<float>();
+  c.w = w.data_ptr();
+  if (du) {
+    need_rows(*du, dh, rows, cols, "dx_out");
+    c.du = du->data_ptr(); c.ld_du = du->stride(0);
+  }
+  if (h) {
+    TORCH_CHECK(b, "the norm's output needs its bias");
+    need_rows(*h, dh, rows, cols, "h");
+    TORCH_CHECK(h->is_contiguous(), "h must be contiguous");
+    need_vector(*b, dh, cols, "pre_bias");
+    c.h = h->data_ptr(); c.b = b->data_ptr();
+  }
+  const bool branch = y.has_value();
+  need_like(grads, dh, dh.scalar_type(), "grads");
+  TORCH_CHECK(grads.numel() == (branch ? 5 : 2) * cols, "grads must be ", shape_text(branch ? 5 : 2, cols));
+  const int64_t step = cols * grads.element_size();
+  char* gp = static_cast<char*>(grads.data_ptr());
+  c.dw = gp; c.db = gp + step;
+  if (branch) {
+    TORCH_CHECK(dy && pw && pb && gate && mean_y && rstd_y, "the branch's tensors go together");
+    kept(*y, "y");
+    need_rows(*dy, dh, rows, cols, "dy");
+    need_floats(*mean_y, dh, rows, "mean_y"); need_floats(*rstd_y, dh, rows, "rstd_y");
+    need_vector(*pw, dh, cols, "post_weight"); need_vector(*pb, dh, cols, "post_bias");
+    need_vector(*gate, dh, cols, "gate");
+    c.y = y->data_ptr(); c.ld_y = y->stride(0);
+    c.dy = dy->data_ptr(); c.ld_dy = dy->stride(0);
+    c.mean_y = mean_y->data_ptr<float>(); c.rstd_y = rstd_y->data_ptr<float>();
+    c.pw = pw->data_ptr(); c.pb = pb->data_ptr(); c.gate = gate->data_ptr();
+    c.dpw = gp + 2 * step; c.dpb = gp + 3 * step; c.dgate = gp + 4 * step;
+  }
+  need_floats(workspace, dh, join_bwd_workspace(rows, cols, branch), "workspace");
+  c.workspace = workspace.data_ptr<float>();
+  const c10::cuda::CUDAGuard g(dh.device());
+  ok(k::join_bwd(c, cur()), branch ? "block_join_bwd" : "layer_norm_bwd_packed");
+}
 }  // namespace
 
 // Launch entry points touch no Python object: the GIL is released while they
@@ -227,6 +432,16 @@ void register_kernels(pybind11::module& m) {
   m.def("ce_sumexp", &ce_sumexp, nogil());
   m.def("ce_loss", &ce_loss, nogil());
   m.def("ce_bwd", &ce_bwd, nogil());
+  m.def("score_fwd", &score_fwd, nogil());
+  m.def("score_merge", &score_merge, nogil());
+  m.def("score_bwd", &score_bwd, nogil());
+  m.def("act_pack_row_bytes", &k::act_pack_row_bytes);
+  m.def("act_pack", &act_pack, nogil());
+  m.def("act_unpack", &act_unpack, nogil());
+  m.def("join_fwd", &join_fwd, nogil());
+  m.def("join_bwd", &join_bwd, nogil());
+  m.def("join_bwd_workspace", &join_bwd_workspace, nogil());
+  m.def("join_max_cols", &k::join_max_cols);
   m.def("grad_sqsum_parts", &grad_sqsum_parts, nogil());
   m.def("grad_sqsum", &grad_sqsum, nogil());
   m.def("adamw_step", &adamw_step, nogil());

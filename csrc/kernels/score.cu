@@ -1,0 +1,588 @@
+// Scores of given tokens from logits (sm_100a): log probability, entropy and the
+// most probable alternatives of every row in one pass, and the gradient of the
+// log probability and the entropy.
+//
+//   m = max z, s = sum e^(z - m), u = sum e^(z - m) (z - m)
+//   log p_t = z_t - m - ln s          H = ln s - u / s
+//   d z_j = a ([j = t] - p_j) - b p_j (ln p_j + H)      a = d log p_t, b = d H
+//
+// Forward: a cluster of 1 to 8 CTAs per row, each thread with running (m, s, u)
+// in FP32 over 16-byte vectors; a logit of -inf adds nothing.  The alternatives
+// need no sort of the row: each thread keeps its largest value and the start of
+// the vector that held it.  The k-th largest of these 256 (value, start) pairs
+// bounds the k-th largest logit from below, and only the k threads at or above
+// it can hold one, so a second look at those threads' vectors collects the few
+// candidates, which one warp sorts.  Equal values go to the lowest index.
+// Ranks of a vocabulary-parallel group exchange one record a row (m, s, u, z_t
+// and their own alternatives) and merge them in rank order.
+#include <cooperative_groups.h>
+
+#include <cmath>
+#include <type_traits>
+
+#include "kernels_api.h"
+#include "rowvec.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace tn5b {
+namespace kernels {
+namespace {
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxTop = 32;       // alternatives a row: one sorted list per warp
+constexpr int kCandidates = 1024;  // 8 KB; more than that takes the selection by rounds
+constexpr int kUnroll = 4;
+constexpr float kLog2e = 1.44269504088896340736f;
+// e^d with d below this is zero in FP32; it also keeps 0 * (-inf) out of u.
+constexpr float kLowest = -200.f;
+
+using Key = unsigned long long;  // order of (value, -index): a larger key comes first
+
+__device__ __forceinline__ unsigned order_of(float v) {
+  v += 0.f;  // -0 and 0 are one value
+  if (v != v) return 0xffffffffu;
+  const unsigned b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(Key key) {
+  const unsigned o = unsigned(key >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);  // NaN's 0xffffffff gives a NaN
+}
+__device__ __forceinline__ Key make_key(float v, unsigned index) {
+  return Key(order_of(v)) << 32 | Key(~index);
+}
+__device__ __forceinline__ unsigned index_of(Key key) { return ~unsigned(key); }
+
+__device__ __forceinline__ Key shfl_xor_key(Key k, int d) { return __shfl_xor_sync(kAllLanes, k, d); }
+// One compare-exchange across lanes: keeps the larger key where `first`.
+__device__ __forceinline__ Key exchange(Key k, int d, bool larger) {
+  const Key o = shfl_xor_key(k, d);
+  return (o > k) == larger ? o : k;
+}
+// Descending over the lanes of a warp.
+__device__ __forceinline__ Key sort_warp(Key k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int d = size >> 1; d; d >>= 1) {
+      const bool descending = size == 32 || (lane & size) == 0;
+      k = exchange(k, d, ((lane & d) == 0) == descending);
+    }
+  }
+  return k;
+}
+// The 32 largest of two descending lists, descending.
+__device__ __forceinline__ Key merge_warp(Key a, Key b) {
+  const int lane = threadIdx.x & 31;
+  const Key r = __shfl_sync(kAllLanes, b, 31 - lane);
+  Key k = a > r ? a : r;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) k = exchange(k, d, (lane & d) == 0);
+  return k;
+}
+
+struct Sums {
+  float m, s, u;
+};
+// Joins b's sums to a's; either may be empty (m = -inf, s = u = 0).
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  Sums r;
+  r.m = max_nan(a.m, b.m);
+  const float base = r.m == -INFINITY ? 0.f : r.m;
+  const float da = fmaxf(a.m - base, kLowest), db = fmaxf(b.m - base, kLowest);
+  const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
+  r.s = a.s * fa + b.s * fb;
+  r.u = (a.u + da * a.s) * fa + (b.u + db * b.s) * fb;
+  return r;
+}
+
+// Where the results of a row go.
+struct Out {
+  float* logprob;    // [rows]
+  float* entropy;    // [rows]
+  float* state;      // [3][rows]: m, ln s, H
+  float* top_value;  // [rows][k]
+  int64_t* top_id;   // [rows][k]
+  float* record;     // [rows][4 + 2k]: m, s, u, z_t, values, ids (ranks of a group), or null
+  int rows, k;
+};
+
+__device__ __forceinline__ void finish_row(const Out& o, int row, Sums a, float picked, int64_t target,
+                                           int64_t vocab_total) {
+  const float nan = __int_as_float(0x7fffffff);
+  float logprob, entropy, m = a.m, ln_s = 0.f;
+  if (!(m < INFINITY)) {  // NaN or +inf among the logits
+    logprob = entropy = m = nan;
+  } else if (m == -INFINITY) {  // nothing left by the mask
+    logprob = -INFINITY;
+    entropy = 0.f;
+  } else {
+    ln_s = logf(a.s);
+    logprob = (picked - m) - ln_s;
+    entropy = ln_s - a.u / a.s;
+  }
+  if (target < 0) logprob = 0.f;
+  if (target >= vocab_total) logprob = nan;
+  o.logprob[row] = logprob;
+  o.entropy[row] = entropy;
+  o.state[row] = m;
+  o.state[o.rows + row] = ln_s;
+  o.state[2 * int64_t(o.rows) + row] = entropy;
+}
+__device__ __forceinline__ float top_logprob(float value, Sums a) {
+  if (a.m == -INFINITY) return -INFINITY;
+  if (!(a.m < INFINITY)) return __int_as_float(0x7fffffff);
+  return (value - a.m) - logf(a.s);
+}
+
+template <typename T>
+struct Vec {  // one 16-byte load
+  static constexpr int kN = 16 / int(sizeof(T));
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float* v) const {
+    const T* h = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = to_float(h[i]);
+  }
+};
+
+// One thread's running state.
+template <bool TOP>
+struct Running {
+  Sums a{-INFINITY, 0.f, 0.f};
+  unsigned best = 0, best_at = 0xffffffffu;  // order_of the largest value, start of its vector
+
+  // N values of a chunk; every COUNT of them begin at index at[i / COUNT].
+  template <int N, int COUNT>
+  __device__ __forceinline__ void add(const float* v, const unsigned* at) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < N / COUNT; ++g) {
+      float t = v[g * COUNT];
+#pragma unroll
+      for (int i = 1; i < COUNT; ++i) t = max_nan(t, v[g * COUNT + i]);
+      if (TOP) {
+        const unsigned o = order_of(t);
+        if (o > best) {
+          best = o;
+          best_at = at[g];
+        }
+      }
+      top = max_nan(top, t);
+    }
+    const float m = max_nan(a.m, top);
+    const float base = m == -INFINITY ? 0.f : m;
+    const float d0 = fmaxf(a.m - base, kLowest);
+    const float f = fast_exp2(d0 * kLog2e);
+    a.u = (a.u + d0 * a.s) * f;
+    a.s *= f;
+    a.m = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = fmaxf(v[i] - base, kLowest);
+      const float e = fast_exp2(d * kLog2e);
+      a.s += e;
+      a.u = fmaf(e, d, a.u);
+    }
+  }
+  __device__ __forceinline__ Key key() const { return best ? Key(best) << 32 | Key(~best_at) : 0; }
+};
+
+// The part of a row that one CTA reads: `head` single values up to a 16-byte
+// boundary, `vectors` vectors, `tail` single values.
+template <typename T>
+struct Part {
+  const T* x;
+  unsigned lo, head, vectors, tail;
+  __device__ __forceinline__ Part(const T* row, unsigned begin, unsigned end) {
+    x = row + begin;
+    lo = begin;
+    const unsigned n = end - begin;
+    const unsigned off = unsigned((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    head = off ? min(n, unsigned(Vec<T>::kN) - off) : 0u;
+    vectors = (n - head) / Vec<T>::kN;
+    tail = n - head - vectors * Vec<T>::kN;
+  }
+  __device__ __forceinline__ unsigned vector_at(unsigned j) const { return head + j * Vec<T>::kN; }
+};
+
+struct TopShared {
+  Key lists[kWarps][32];
+  Key candidates[kCandidates];
+  Key best[kWarps];
+  unsigned active[kThreads];
+  unsigned active_count, count;
+};
+
+// Descending list of the CTA's 32 best, of which the first k count, in every
+// lane of warp 0 (and in sh.lists[0]).
+template <typename T>
+__device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, TopShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) sh.active_count = sh.count = 0;
+  Key list = sort_warp(own);
+  sh.lists[warp][lane] = list;
+  __syncthreads();
+#pragma unroll
+  for (int half = kWarps / 2; half; half >>= 1) {
+    if (warp < half) {
+      list = merge_warp(list, sh.lists[warp + half][lane]);
+      sh.lists[warp][lane] = list;
+    }
+    __syncthreads();
+  }
+  const Key bound = sh.lists[0][k - 1];
+  if (own >= bound) sh.active[atomicAdd(&sh.active_count, 1u)] = tid;
+  __syncthreads();
+
+  // Visits every value whose (value, start of vector) reaches the bound; its own
+  // key is handed on.  Items: the active threads' vectors, then single values.
+  const unsigned per = (part.vectors + kThreads - 1) / kThreads;
+  const unsigned scalars = part.head + part.tail;
+  const unsigned items = sh.active_count * per;
+  auto visit = [&](auto&& take) {
+    for (unsigned i = tid; i < items + scalars; i += kThreads) {
+      if (i < items) {
+        const unsigned a = i / per, j = sh.active[a] + (i - a * per) * kThreads;
+        if (j >= part.vectors) continue;
+        const unsigned at = part.vector_at(j);
+        Vec<T> vec;
+        float v[Vec<T>::kN];
+        vec.load(part.x + at);
+        vec.get(v);
+#pragma unroll
+        for (int e = 0; e < Vec<T>::kN; ++e)
+          if (make_key(v[e], part.lo + at) >= bound) take(make_key(v[e], part.lo + at + e));
+      } else {
+        const unsigned c = i - items;
+        const unsigned at = c < part.head ? c : part.vector_at(part.vectors) + (c - part.head);
+        const Key key = make_key(to_float(part.x[at]), part.lo + at);
+        if (key >= bound) take(key);
+      }
+    }
+  };
+  visit([&](Key key) {
+    const unsigned at = atomicAdd(&sh.count, 1u);
+    if (at < kCandidates) sh.candidates[at] = key;
+  });
+  __syncthreads();
+  const unsigned n = sh.count;
+  if (n <= kCandidates) {
+    if (warp == 0) {
+      list = 0;
+      for (unsigned at = 0; at < n; at += 32) {
+        const Key next = sort_warp(at + lane < n ? sh.candidates[at + lane] : 0);
+        list = at ? merge_warp(list, next) : next;
+      }
+      sh.lists[0][lane] = list;
+    }
+  } else {
+    // Many candidates in few threads' vectors: the k largest one after another.
+    Key below = ~Key(0);
+    for (int r = 0; r < k; ++r) {
+      Key best = 0;
+      visit([&](Key key) {
+        if (key < below && key > best) best = key;
+      });
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        const Key o = shfl_xor_key(best, d);
+        if (o > best) best = o;
+      }
+      if (lane == 0) sh.best[warp] = best;
+      __syncthreads();
+      best = sh.best[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) best = best > sh.best[w] ? best : sh.best[w];
+      below = best;
+      if (tid == 0) sh.lists[0][r] = best;
+      __syncthreads();
+    }
+    if (warp == 0 && lane >= k) sh.lists[0][lane] = 0;
+  }
+  __syncthreads();
+}
+
+// grid = rows * C CTAs in clusters of C; the cluster's CTAs take `chunk` columns each.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_t ld, unsigned vocab,
+                                                         const int64_t* targets, int64_t start,
+                                                         int64_t vocab_total, unsigned chunk, Out o) {
+  __shared__ Sums warp_sums[kWarps];
+  __shared__ Sums block_sums;
+  __shared__ std::conditional_t<TOP, TopShared, int> sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int row = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* x = logits + int64_t(row) * ld;
+  const unsigned begin = min(vocab, rank * chunk), end = min(vocab, begin + chunk);
+  const Part<T> part(x, begin, end);
+  constexpr int kN = Vec<T>::kN;
+
+  Running<TOP> run;
+  if (unsigned(tid) < part.head) {
+    const float v = to_float(part.x[tid]);
+    const unsigned at = part.lo + tid;
+    run.template add<1, 1>(&v, &at);
+  }
+  unsigned j = tid;
+  for (; j + (kUnroll - 1) * kThreads < part.vectors; j += kUnroll * kThreads) {
+    Vec<T> vec[kUnroll];
+    float v[kUnroll * kN];
+    unsigned at[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) vec[i].load(part.x + part.vector_at(j + i * kThreads));
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      vec[i].get(v + i * kN);
+      at[i] = part.lo + part.vector_at(j + i * kThreads);
+    }
+    run.template add<kUnroll * kN, kN>(v, at);
+  }
+  for (; j < part.vectors; j += kThreads) {
+    Vec<T> vec;
+    float v[kN];
+    const unsigned at = part.lo + part.vector_at(j);
+    vec.load(part.x + part.vector_at(j));
+    vec.get(v);
+    run.template add<kN, kN>(v, &at);
+  }
+  if (unsigned(tid) < part.tail) {
+    const unsigned i = part.vector_at(part.vectors) + tid;
+    const float v = to_float(part.x[i]);
+    const unsigned at = part.lo + i;
+    run.template add<1, 1>(&v, &at);
+  }
+
+  Sums a = run.a;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    Sums b;
+    b.m = __shfl_xor_sync(kAllLanes, a.m, d);
+    b.s = __shfl_xor_sync(kAllLanes, a.s, d);
+    b.u = __shfl_xor_sync(kAllLanes, a.u, d);
+    // The lower lane's sums come first on both sides, so both get the same bits.
+    a = lane & d ? join(b, a) : join(a, b);
+  }
+  if (lane == 0) warp_sums[warp] = a;
+  if constexpr (TOP) block_top(part, run.key(), o.k, sh);  // synchronises
+  else __syncthreads();
+  if (tid == 0) {
+    a = warp_sums[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) a = join(a, warp_sums[w]);
+    block_sums = a;
+  }
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+  if (rank == 0 && warp == 0) {
+    a = block_sums;
+    for (unsigned r = 1; r < C; ++r) a = join(a, *cluster.map_shared_rank(&block_sums, r));
+    Key list = 0;
+    if constexpr (TOP) {
+      list = sh.lists[0][lane];
+      for (unsigned r = 1; r < C; ++r) list = merge_warp(list, cluster.map_shared_rank(&sh.lists[0][0], r)[lane]);
+    }
+    const int64_t target = targets[row], local = target - start;
+    const float picked = local >= 0 && local < vocab ? to_float(x[local]) : 0.f;
+    if (o.record) {
+      float* rec = o.record + int64_t(row) * (4 + 2 * o.k);
+      if (lane == 0) {
+        rec[0] = a.m;
+        rec[1] = a.s;
+        rec[2] = a.u;
+        rec[3] = picked;
+      }
+      if (TOP && lane < o.k) {
+        rec[4 + lane] = value_of(list);
+        rec[4 + o.k + lane] = __int_as_float(int(index_of(list) + unsigned(start)));
+      }
+    } else {
+      if (lane == 0) finish_row(o, row, a, picked, target, vocab_total);
+      if (TOP && lane < o.k) {
+        o.top_value[int64_t(row) * o.k + lane] = top_logprob(value_of(list), a);
+        o.top_id[int64_t(row) * o.k + lane] = start + index_of(list);
+      }
+    }
+  }
+  if (C > 1) cluster.sync();  // shared memory stays until rank 0 has read it
+}
+
+// Records of `parts` ranks, [parts][rows][4 + 2k], one warp a row.
+__global__ void __launch_bounds__(kThreads) score_merge_kernel(const float* records, int parts, int64_t vocab,
+                                                               const int64_t* targets, Out o) {
+  const int row = blockIdx.x * kWarps + threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (row >= o.rows) return;
+  const int64_t target = targets[row];
+  Sums a{-INFINITY, 0.f, 0.f};
+  float picked = 0.f;
+  Key list = 0;
+  for (int p = 0; p < parts; ++p) {
+    const float* rec = records + (int64_t(p) * o.rows + row) * (4 + 2 * o.k);
+    a = join(a, Sums{rec[0], rec[1], rec[2]});
+    if (target >= p * vocab && target < (p + 1) * vocab) picked = rec[3];
+    if (o.k) {
+      const Key next = lane < o.k ? make_key(rec[4 + lane], unsigned(__float_as_int(rec[4 + o.k + lane]))) : 0;
+      list = merge_warp(list, next);
+    }
+  }
+  if (lane == 0) finish_row(o, row, a, picked, target, parts * vocab);
+  if (lane < o.k) {
+    o.top_value[int64_t(row) * o.k + lane] = top_logprob(value_of(list), a);
+    o.top_id[int64_t(row) * o.k + lane] = index_of(list);
+  }
+}
+
+// One CTA per `kUnroll` vectors of its threads along a row.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, int64_t ld, unsigned vocab,
+                                                             const int64_t* targets, int64_t start,
+                                                             int64_t vocab_total, const float* state, int rows,
+                                                             const float* dlogprob, const float* dentropy, T* out,
+                                                             int64_t ld_out, unsigned blocks) {
+  constexpr int kN = Vec<T>::kN;
+  const int row = blockIdx.x / blocks;
+  const unsigned block = blockIdx.x - unsigned(row) * blocks;
+  const float m = state[row], ln_s = state[rows + row], H = state[2 * int64_t(rows) + row];
+  const int64_t target = targets[row];
+  float a = target >= 0 ? dlogprob[row] : 0.f;
+  const float b = dentropy ? dentropy[row] : 0.f;
+  if (target >= vocab_total || m != m) a = __int_as_float(0x7fffffff);
+  const bool empty = m == -INFINITY;
+  const int64_t local = target - start;
+  const unsigned at = local >= 0 && local < vocab ? unsigned(local) : 0xffffffffu;
+  auto gradient = [&](float z, unsigned i) {
+    const float l = fmaxf((z - m) - ln_s, kLowest);
+    const float p = fast_exp2(l * kLog2e);
+    float g = -p * (a + b * (l + H));
+    if (i == at) g += a;
+    return empty ? 0.f : g;
+  };
+  const T* x = logits + int64_t(row) * ld;
+  T* y = out + int64_t(row) * ld_out;
+  if (VEC) {  // both rows are off a 16-byte boundary by the same amount
+    const Part<T> part(x, 0, vocab);
+    Vec<T> vec[kUnroll];
+    const unsigned j0 = block * (kUnroll * kThreads) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (j0 + i * kThreads < part.vectors) vec[i].load(x + part.vector_at(j0 + i * kThreads));
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const unsigned j = j0 + i * kThreads;
+      if (j >= part.vectors) break;
+      const unsigned c = part.vector_at(j);
+      float v[kN];
+      vec[i].get(v);
+      T* h = reinterpret_cast<T*>(&vec[i].raw);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) h[e] = from_float<T>(gradient(v[e], c + e));
+      *reinterpret_cast<uint4*>(y + c) = vec[i].raw;
+    }
+    if (block == 0 && threadIdx.x < part.head + part.tail) {
+      const unsigned c = threadIdx.x < part.head ? threadIdx.x
+                                                 : part.vector_at(part.vectors) + (threadIdx.x - part.head);
+      y[c] = from_float<T>(gradient(to_float(x[c]), c));
+    }
+  } else {
+    const unsigned c0 = block * (kUnroll * kThreads * kN) + threadIdx.x;
+#pragma unroll 4
+    for (int i = 0; i < kUnroll * kN; ++i) {
+      const unsigned c = c0 + i * kThreads;
+      if (c < vocab) y[c] = from_float<T>(gradient(to_float(x[c]), c));
+    }
+  }
+}
+
+template <typename T, bool TOP>
+int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
+                 int64_t vocab_total, const Out& o, cudaStream_t s) {
+  // A row is split over a cluster while the rows alone leave SMs idle.
+  unsigned C = 1;
+  while (C < 8 && int64_t(o.rows) * C * 2 <= 148 * 4 && vocab / (2 * C) >= 4096) C *= 2;
+  const unsigned step = Vec<T>::kN;  // every part is off a 16-byte boundary by what the row is
+  const unsigned chunk = C == 1 ? vocab : ((vocab + C - 1) / C + step - 1) / step * step;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(o.rows) * C);
+  config.blockDim = dim3(kThreads);
+  config.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return int(cudaLaunchKernelEx(&config, score_kernel<T, TOP>, static_cast<const T*>(logits), ld, vocab, targets,
+                                start, vocab_total, chunk, o));
+}
+template <typename T>
+int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
+                int64_t vocab_total, const Out& o, cudaStream_t s) {
+  return o.k ? launch_score<T, true>(logits, ld, vocab, targets, start, vocab_total, o, s)
+             : launch_score<T, false>(logits, ld, vocab, targets, start, vocab_total, o, s);
+}
+template <typename T>
+int score_bwd_typed(const void* logits, int64_t ld, int rows, unsigned vocab, const int64_t* targets, int64_t start,
+                    int64_t vocab_total, const float* state, const float* dlogprob, const float* dentropy, void* out,
+                    int64_t ld_out, cudaStream_t s) {
+  constexpr int64_t kE = sizeof(T), kN = Vec<T>::kN;
+  const unsigned span = kThreads * kUnroll * unsigned(kN);
+  const unsigned blocks = (vocab + span - 1) / span;
+  if (int64_t(rows) * blocks > 0x7fffffff) return -1;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(logits), b = reinterpret_cast<uintptr_t>(out);
+  const bool vec = (a & 15) == (b & 15) && ((ld - ld_out) * kE) % 16 == 0;
+  auto launch = [&](auto kernel) {
+    kernel<<<unsigned(rows) * blocks, kThreads, 0, s>>>(static_cast<const T*>(logits), ld, vocab, targets, start,
+                                                        vocab_total, state, rows, dlogprob, dentropy,
+                                                        static_cast<T*>(out), ld_out, blocks);
+  };
+  vec ? launch(score_bwd_kernel<T, true>) : launch(score_bwd_kernel<T, false>);
+  return int(cudaGetLastError());
+}
+bool sizes_fit(int64_t rows, int64_t vocab, int64_t vocab_total) {
+  // Ids travel as 32-bit integers; a launch has rows * 8 CTAs at most.
+  return rows > 0 && vocab > 0 && rows <= 0x7fffffff / 8 && vocab_total <= 0x7fffffff;
+}
+}  // namespace
+
+int score_fwd(const void* logits, int type, int64_t ld, int64_t rows, int64_t vocab, const int64_t* targets,
+              int64_t start, int64_t vocab_total, int k, float* logprob, float* entropy, float* state,
+              float* top_value, int64_t* top_id, float* record, cudaStream_t s) {
+  if (!sizes_fit(rows, vocab, vocab_total) || k < 0 || k > kMaxTop || k > vocab) return -1;
+  const Out o{logprob, entropy, state, top_value, top_id, record, int(rows), k};
+  const unsigned v = unsigned(vocab);
+  if (type == kTypeBF16) return score_typed<__nv_bfloat16>(logits, ld, v, targets, start, vocab_total, o, s);
+  if (type == kTypeFP16) return score_typed<__half>(logits, ld, v, targets, start, vocab_total, o, s);
+  if (type == kTypeFP32) return score_typed<float>(logits, ld, v, targets, start, vocab_total, o, s);
+  return -1;
+}
+int score_merge(const float* records, int parts, int64_t rows, int64_t vocab, const int64_t* targets, int k,
+                float* logprob, float* entropy, float* state, float* top_value, int64_t* top_id, cudaStream_t s) {
+  if (!sizes_fit(rows, vocab, parts * vocab) || parts < 1 || k < 0 || k > kMaxTop) return -1;
+  const Out o{logprob, entropy, state, top_value, top_id, nullptr, int(rows), k};
+  score_merge_kernel<<<unsigned((rows + kWarps - 1) / kWarps), kThreads, 0, s>>>(records, parts, vocab, targets, o);
+  return int(cudaGetLastError());
+}
+int score_bwd(const void* logits, int type, int64_t ld, int64_t rows, int64_t vocab, const int64_t* targets,
+              int64_t start, int64_t vocab_total, const float* state, const float* dlogprob, const float* dentropy,
+              void* out, int64_t ld_out, cudaStream_t s) {
+  if (!sizes_fit(rows, vocab, vocab_total)) return -1;
+  const unsigned v = unsigned(vocab);
+  const int r = int(rows);
+  if (type == kTypeBF16)
+    return score_bwd_typed<__nv_bfloat16>(logits, ld, r, v, targets, start, vocab_total, state, dlogprob, dentropy,
+                                          out, ld_out, s);
+  if (type == kTypeFP16)
+    return score_bwd_typed<__half>(logits, ld, r, v, targets, start, vocab_total, state, dlogprob, dentropy, out,
+                                   ld_out, s);
+  if (type == kTypeFP32)
+    return score_bwd_typed<float>(logits, ld, r, v, targets, start, vocab_total, state, dlogprob, dentropy, out,
+                                  ld_out, s);
+  return -1;
+}
+
+}  // namespace kernels
+}  // namespace tn5b

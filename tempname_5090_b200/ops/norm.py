@@ -1,14 +1,23 @@
-"""LayerNorm forward/backward, GeLU backward and column sums.
+"""LayerNorm forward/backward, the joint of two blocks, GeLU backward and column sums.
 
 CUDA tensors: native sm_100a kernels.  CPU tensors: the same math in torch
 (test oracle path).  Semantics: F.layer_norm in FP32 on BF16 storage.
+
+The joint (`block_join_fwd`) is what stands between two branches of a network
+that normalises before and after each of them: the norm of the branch's output,
+its gate, the scaled residual and the norm of the next branch's input, in one
+pass.  Its gradient (`block_join_bwd`) and LayerNorm's (`layer_norm_bwd_packed`)
+also read inputs kept in 8 bits (ops/actpack.py).
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from .._native import count_launch, lib
+from .actpack import Packed8, _values
 
 
 def layer_norm_fwd(x, weight, bias, eps, out=None):
@@ -89,3 +98,219 @@ def column_sum(g, out=None, workspace=None):
         out.copy_(s)
         return out
     return s
+
+
+# ------------------------------------------------------------------ block joint
+JOIN_DTYPES = (torch.bfloat16, torch.float32)
+JOIN_MAX_COLS = 8192
+
+
+class JoinGrads(NamedTuple):
+    dx: torch.Tensor            # [rows, H], of the residual stream's input
+    dy: torch.Tensor            # [rows, H], of the branch's output
+    dpost_weight: torch.Tensor  # [H] each
+    dpost_bias: torch.Tensor
+    dgate: torch.Tensor
+    dpre_weight: torch.Tensor
+    dpre_bias: torch.Tensor
+    h: torch.Tensor | None      # the next branch's input again, where it was asked for
+
+
+def _check_matrix(name, t, like, shape, own_rows=False):
+    if t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)} of {like.dtype} on {like.device}")
+    if shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} needs contiguous rows")
+    if own_rows and shape[0] > 1 and t.stride(0) < shape[1]:
+        raise ValueError(f"{name} needs rows of its own")
+
+
+def _check_vectors(like, cols, **vectors):
+    for name, t in vectors.items():
+        if t.dtype != like.dtype or t.device != like.device or t.shape != (cols,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous ({cols},) of {like.dtype} on {like.device}")
+
+
+def _check_stats(like, shape, **stats):
+    for name, t in stats.items():
+        if t.dtype != torch.float32 or t.device != like.device or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous FP32 {tuple(shape)} on {like.device}")
+
+
+def _check_first(name, t):
+    if t.dim() != 2 or t.dtype not in JOIN_DTYPES:
+        raise ValueError(f"{name} must be a BF16 or FP32 matrix")
+    if not 1 <= t.shape[1] <= JOIN_MAX_COLS:
+        raise ValueError(f"the hidden size must be between 1 and {JOIN_MAX_COLS}")
+
+
+def _check_kept(name, t, like, shape):
+    if isinstance(t, Packed8):
+        if t.shape != shape or t.device != like.device:
+            raise ValueError(f"{name} must be the packed form of {tuple(shape)} on {like.device}")
+    else:
+        _check_matrix(name, t, like, shape)
+
+
+@torch.no_grad()
+def block_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps, residual_scale=1.0, out=None):
+    """Returns (x_out, h, stats) for the residual stream x and a branch's output y, [rows, H]:
+
+        x_out = residual_scale * x + gate * LayerNorm(y; post_weight, post_bias)
+        h     = LayerNorm(x_out; pre_weight, pre_bias)
+
+    gate and the norms' parameters are [H].  BF16 or FP32, H up to 8192, any row
+    strides; h may be written into `out` (a row-strided view is allowed).  h is
+    computed from x_out before its rounding to the storage type.  `stats` (FP32
+    [4, rows]: mean and reciprocal deviation of y, then of x_out) is for the gradient.
+    """
+    _check_first("x", x)
+    rows, H = x.shape
+    _check_matrix("x", x, x, x.shape)
+    _check_matrix("y", y, x, x.shape)
+    _check_vectors(x, H, post_weight=post_weight, post_bias=post_bias, gate=gate, pre_weight=pre_weight,
+                   pre_bias=pre_bias)
+    if out is not None:
+        _check_matrix("out", out, x, x.shape, own_rows=True)
+    if x.is_cuda:
+        x_out = torch.empty((rows, H), dtype=x.dtype, device=x.device)
+        h = torch.empty_like(x_out) if out is None else out
+        stats = torch.empty((4, rows), dtype=torch.float32, device=x.device)
+        if rows:
+            lib().join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, x_out, h, stats,
+                           float(residual_scale), float(eps))
+            count_launch()
+        return x_out, h, stats
+    yhat, mean_y, rstd_y = _normed(y.float(), eps)
+    u = residual_scale * x.float() + gate.float() * (yhat * post_weight.float() + post_bias.float())
+    uhat, mean_u, rstd_u = _normed(u, eps)
+    h = (uhat * pre_weight.float() + pre_bias.float()).to(x.dtype)
+    if out is not None:
+        out.copy_(h)
+        h = out
+    return u.to(x.dtype), h, torch.stack([mean_y, rstd_y, mean_u, rstd_u])
+
+
+def _normed(v, eps):
+    mean = v.mean(1)
+    rstd = torch.rsqrt(v.var(1, unbiased=False) + eps)
+    return (v - mean[:, None]) * rstd[:, None], mean, rstd
+
+
+def _kept_float(t):
+    return _values(t) if isinstance(t, Packed8) else t.float()
+
+
+def _norm_input_grad(g, hat, rstd):
+    return rstd[:, None] * (g - g.mean(1, keepdim=True) - hat * (g * hat).mean(1, keepdim=True))
+
+
+def _join_workspace(workspace, rows, H, branch, device):
+    need = lib().join_bwd_workspace(rows, H, branch)
+    if workspace is None or workspace.numel() < need:
+        workspace = torch.empty(need, dtype=torch.float32, device=device)
+    return workspace
+
+
+@torch.no_grad()
+def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, residual_scale=1.0,
+                   pre_bias=None, workspace=None, out=None) -> JoinGrads:
+    """Gradients of `block_join_fwd` from that of h and (or None) of x_out.
+
+    x_out and y are the forward's tensors, or both their packed 8-bit forms.  dy may
+    be written into `out` (a row-strided view is allowed).  With `pre_bias` given, h is
+    computed again from x_out and returned too.  `workspace` (FP32) is used where it
+    is large enough.  Gradients of x_out and h join in FP32; parameter gradients are
+    sums over the rows in a fixed order.
+    """
+    _check_first("dh", dh)
+    rows, H = dh.shape
+    _check_matrix("dh", dh, dh, dh.shape)
+    if dx_out is not None:
+        _check_matrix("dx_out", dx_out, dh, dh.shape)
+    if isinstance(x_out, Packed8) != isinstance(y, Packed8):
+        raise ValueError("x_out and y are kept in the same form")
+    _check_kept("x_out", x_out, dh, dh.shape)
+    _check_kept("y", y, dh, dh.shape)
+    _check_stats(dh, (4, rows), stats=stats)
+    _check_vectors(dh, H, post_weight=post_weight, post_bias=post_bias, gate=gate, pre_weight=pre_weight)
+    if pre_bias is not None:
+        _check_vectors(dh, H, pre_bias=pre_bias)
+    if out is not None:
+        _check_matrix("out", out, dh, dh.shape, own_rows=True)
+    if dh.is_cuda:
+        dx = torch.empty((rows, H), dtype=dh.dtype, device=dh.device)
+        dy = torch.empty_like(dx) if out is None else out
+        h = None if pre_bias is None else torch.empty_like(dx)
+        grads = torch.empty((5, H), dtype=dh.dtype, device=dh.device)
+        if rows:
+            packed = isinstance(x_out, Packed8)
+            lib().join_bwd(dh, dx_out, x_out.data if packed else x_out, y.data if packed else y, stats[2], stats[3],
+                           stats[0], stats[1], post_weight, post_bias, gate, pre_weight, pre_bias, dx, dy, h, grads,
+                           _join_workspace(workspace, rows, H, True, dh.device), float(residual_scale))
+            count_launch(2)
+        else:
+            grads.zero_()
+        return JoinGrads(dx, dy, grads[2], grads[3], grads[4], grads[0], grads[1], h)
+    mean_y, rstd_y, mean_u, rstd_u = stats
+    uhat = (_kept_float(x_out) - mean_u[:, None]) * rstd_u[:, None]
+    yhat = (_kept_float(y) - mean_y[:, None]) * rstd_y[:, None]
+    dhf, pw, g = dh.float(), post_weight.float(), gate.float()
+    dt = _norm_input_grad(dhf * pre_weight.float(), uhat, rstd_u)
+    if dx_out is not None:
+        dt = dt + dx_out.float()
+    dn = dt * g
+    dy = _norm_input_grad(dn * pw, yhat, rstd_y).to(dh.dtype)
+    if out is not None:
+        out.copy_(dy)
+        dy = out
+    h = None if pre_bias is None else (uhat * pre_weight.float() + pre_bias.float()).to(dh.dtype)
+    return JoinGrads((residual_scale * dt).to(dh.dtype), dy, (dn * yhat).sum(0).to(dh.dtype), dn.sum(0).to(dh.dtype),
+                     (dt * (yhat * pw + post_bias.float())).sum(0).to(dh.dtype),
+                     (dhf * uhat).sum(0).to(dh.dtype), dhf.sum(0).to(dh.dtype), h)
+
+
+@torch.no_grad()
+def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, workspace=None, out=None):
+    """LayerNorm's gradient from its input kept in 8 bits (x: Packed8) and the
+    statistics of the forward pass.  Returns (dx, dweight, dbias, y): dx includes
+    dres when given (joined in FP32) and is written into `out` when given; y is the
+    norm's output again when `bias` is given (the weight gradient of the product that
+    follows reads it), else None.
+    """
+    _check_first("dy", dy)
+    rows, H = dy.shape
+    _check_matrix("dy", dy, dy, dy.shape)
+    if not isinstance(x, Packed8):
+        raise ValueError("x must be a Packed8")
+    _check_kept("x", x, dy, dy.shape)
+    _check_stats(dy, (rows,), mean=mean, rstd=rstd)
+    _check_vectors(dy, H, weight=weight)
+    if bias is not None:
+        _check_vectors(dy, H, bias=bias)
+    if dres is not None:
+        _check_matrix("dres", dres, dy, dy.shape)
+    if out is not None:
+        _check_matrix("out", out, dy, dy.shape, own_rows=True)
+    if dy.is_cuda:
+        dx = torch.empty((rows, H), dtype=dy.dtype, device=dy.device) if out is None else out
+        y = None if bias is None else torch.empty((rows, H), dtype=dy.dtype, device=dy.device)
+        grads = torch.empty((2, H), dtype=dy.dtype, device=dy.device)
+        if rows:
+            lib().join_bwd(dy, dres, x.data, None, mean, rstd, None, None, None, None, None, weight, bias, dx, None, y,
+                           grads, _join_workspace(workspace, rows, H, False, dy.device), 1.0)
+            count_launch(2)
+        else:
+            grads.zero_()
+        return dx, grads[0], grads[1], y
+    hat = (_values(x) - mean[:, None]) * rstd[:, None]
+    g = dy.float()
+    dx = _norm_input_grad(g * weight.float(), hat, rstd)
+    if dres is not None:
+        dx = dx + dres.float()
+    dx = dx.to(dy.dtype)
+    if out is not None:
+        out.copy_(dx)
+        dx = out
+    y = None if bias is None else (hat * weight.float() + bias.float()).to(dy.dtype)
+    return dx, (g * hat).sum(0).to(dy.dtype), g.sum(0).to(dy.dtype), y
