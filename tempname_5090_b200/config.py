@@ -5,6 +5,10 @@
 (micro-batch 4, vocab 50304, AdamW lr 1e-4).  Both give 8192 tokens per step.
 Validation rules follow model.py:20-47 and parameter counting model.py:50-59,
 extended to TP size 1 (the reference requires W >= 2 for its operator only).
+
+Two optional keys choose the blocks: `block_norm` ("pre", the default, or
+"sandwich": a norm and a per-channel gate after each branch too) and
+`residual_scale` (sandwich blocks: x -> residual_scale * x + gate * norm(branch)).
 """
 from __future__ import annotations
 
@@ -20,6 +24,9 @@ ARMS = ("flux", "flux_taco", "flux_taco_interleaved", "flux_taco_interleaved_arr
 INTEGER_KEYS = tuple(REFERENCE_DEFAULT)
 FLOAT_KEYS = (("learning_rate", 1e-4), ("weight_decay", 0.01), ("max_grad_norm", 1.0),
               ("layer_norm_epsilon", 1e-5))
+
+
+BLOCK_NORMS = ("pre", "sandwich")
 
 
 def validate_config(config: dict, world_size: int = 8) -> dict:
@@ -48,6 +55,15 @@ def validate_config(config: dict, world_size: int = 8) -> dict:
         if value < 0 or (key in ("learning_rate", "max_grad_norm", "layer_norm_epsilon") and value == 0):
             raise ValueError(f"invalid {key}")
         result[key] = float(value)
+    if result.get("block_norm", "pre") not in BLOCK_NORMS:
+        raise ValueError(f"block_norm must be one of {BLOCK_NORMS}")
+    if "residual_scale" in result:
+        value = result["residual_scale"]
+        if isinstance(value, bool) or not isinstance(value, (int, float)) or not math.isfinite(value):
+            raise ValueError("residual_scale must be finite")
+        if result.get("block_norm", "pre") != "sandwich":
+            raise ValueError("residual_scale belongs to sandwich blocks")
+        result["residual_scale"] = float(value)
     return result
 
 
@@ -56,6 +72,9 @@ def parameter_counts(config: dict, world_size: int = 8) -> dict:
     h, f, v, s, layers = (c[k] for k in ("hidden", "ffn", "vocab", "sequence", "layers"))
     logical = v * h + s * h + layers * (4 * h * h + 2 * h * f + 9 * h + f) + 2 * h
     replicated = s * h + layers * 6 * h + 2 * h
+    if c.get("block_norm") == "sandwich":  # post-norm weight, bias and gate of both branches
+        logical += layers * 6 * h
+        replicated += layers * 6 * h
     sharded = logical - replicated
     return dict(logical_parameters=logical, replicated_parameters=replicated,
                 sharded_parameters=sharded,

@@ -19,6 +19,12 @@ AG->GEMM / GEMM->RS operators, saves exactly the activations the backward
 needs, and writes every gradient straight into one flat BF16 gradient buffer
 (weight gradients are tcgen05 GEMM outputs, no extra copies).  Forward
 arithmetic order matches the reference: value = (value + RowLinear(...)) + bias.
+Two choices beside the reference's: `block_norm="sandwich"` in the configuration
+gives every branch a norm and a gate after it as well (layers.i.{attn,mlp}_post_
+{weight,bias} and {attn,mlp}_gate, replicated), with the joint of two branches as
+one kernel; `kept="e4m3"` keeps the tape in 8 bits (ops/actpack.py): residual
+stream, branch outputs, QKV and the MLP's pre-activation, from which the backward
+pass computes the norms' and the activation's outputs and the attention again.
 All parameters live in one flat BF16 buffer ordered [sharded matrices |
 sharded vectors | replicated matrices | replicated vectors] so the optimizer
 is two fused launches.
@@ -32,6 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from ..config import parameter_counts, validate_config
+from ..ops import actpack as K
 from ..ops import attention as A
 from ..ops import embedding as E
 from ..ops import gemm as G
@@ -84,6 +91,10 @@ def param_specs(c: dict, world: int) -> list:
             ParamSpec(f"{p}.fc2_weight", (h, f // world), False, "normal", small, f"{p}fc2w"),
             ParamSpec(f"{p}.fc2_bias", (h,), True, "zero", 0.0, f"{p}fc2b"),
         ]
+        if c.get("block_norm") == "sandwich":
+            for branch in ("attn", "mlp"):
+                for name, init in (("post_weight", "one"), ("post_bias", "zero"), ("gate", "one")):
+                    specs.append(ParamSpec(f"{p}.{branch}_{name}", (h,), True, init, 0.0, f"{p}{branch}{name}"))
     specs.append(ParamSpec("final_weight", (h,), True, "one", 0.0, "final_ln_w"))
     specs.append(ParamSpec("final_bias", (h,), True, "zero", 0.0, "final_ln_b"))
     return specs
@@ -152,7 +163,9 @@ class GPT:
 
     def __init__(self, config: dict, arm: str = "flux", group=None, device="cuda", seed: int = 1234,
                  transport: str = "nvlink", execution_plan: dict | None = None, init: bool = True,
-                 timeout_ns: int = 10_000_000_000):
+                 timeout_ns: int = 10_000_000_000, kept: str = "bf16"):
+        if kept not in ("bf16", "e4m3"):
+            raise ValueError("kept must be 'bf16' or 'e4m3'")
         plans = None
         if execution_plan is not None:
             plans = execution_plan.get("roles", execution_plan)
@@ -161,6 +174,9 @@ class GPT:
         self.world, self.rank = self.tp.world, self.tp.rank
         self.config = validate_config(config, self.world)
         self.arm = arm
+        self.kept = kept
+        self.sandwich = self.config.get("block_norm") == "sandwich"
+        self.residual_scale = self.config.get("residual_scale", 1.0)
         self.device = torch.device(device)
         self.seed = seed
         self.specs = param_specs(self.config, self.world)
@@ -209,6 +225,12 @@ class GPT:
 
     # ------------------------------------------------------------- forward
     def _forward(self, tokens, targets, keep: bool, loss_scale: float):
+        logits, trunk = self._logits(tokens, targets, keep)
+        loss, ce_state = CE.forward(logits, targets, self.tp.group, self.rank, self.world, scale=loss_scale / self.M)
+        return loss, (tokens, targets, trunk, logits, ce_state) if keep else None
+
+    def _logits(self, tokens, targets, keep: bool):
+        """This rank's logits [M, V/W] and the tape of the layers (when `keep`)."""
         c, tp = self.config, self.tp
         M, Ml, h, lh = self.M, self.Ml, self.h, self.lh
         if tokens.shape != (M,) or targets.shape != (M,):
@@ -219,6 +241,11 @@ class GPT:
         x = tp.scatter_sum(contrib)
         E.add_position(x, self.p["position"], row0)
         saved = []
+        if self.sandwich:
+            lnf, first = self._sandwich_forward(x, saved, keep)
+            logits, lnf_full = tp.ag_linear(("head", 0), lnf, self.p["embedding"])
+            self.forward_calls += 1
+            return logits, (saved, first, None, None, lnf_full)
         for i in range(c["layers"]):
             with tracing.scope(f"gpt.layer{i}.forward"):
                 x = self._layer_forward(i, x, saved, keep)
@@ -226,10 +253,29 @@ class GPT:
         buf = tp.ag_input(("head", 0), M, self.h, self.Vl, x.is_cuda)
         lnf, meanf, rstdf = N.layer_norm_fwd(x_final, self.p["final_weight"], self.p["final_bias"], self.eps, out=buf)
         logits, lnf_full = tp.ag_linear(("head", 0), lnf, self.p["embedding"])
-        loss, ce_state = CE.forward(logits, targets, tp.group, self.rank, self.world, scale=loss_scale / M)
         self.forward_calls += 1
-        tape = (tokens, targets, saved, x_final, meanf, rstdf, lnf_full, logits, ce_state) if keep else None
-        return loss, tape
+        return logits, (saved, x_final, meanf, rstdf, lnf_full)
+
+    # ------------------------------------------------------ the tape in 8 bits
+    def _keep(self, t):
+        return K.pack(t) if self.kept == "e4m3" else t
+
+    def _keep_normed(self, full):
+        """A norm's gathered output: the backward pass computes it again on one rank;
+        with TP it lies in the fused operator's gather buffer anyway."""
+        return None if self.kept == "e4m3" and self.world == 1 else full
+
+    def _attention_again(self, qkv, attn, lse):
+        """(qkv, attn, lse) for the attention's backward pass.  From a kept QKV the
+        forward is run again, so that output, LSE and gradient belong together."""
+        if not isinstance(qkv, K.Packed8):
+            return qkv, attn, lse
+        qkv = K.unpack(qkv)
+        attn, lse = A.forward(qkv, self.config["micro_batch"], self.config["sequence"], self.lh)
+        return qkv, attn, lse
+
+    def _mlp_again(self, pre, act):
+        return K.unpack_gelu(pre) if isinstance(pre, K.Packed8) else (pre, act)
 
     def _layer_forward(self, i, x, saved, keep):
         """One transformer block forward (pre-LN); appends its tape when `keep`."""
@@ -254,9 +300,26 @@ class GPT:
         act, ln2_full = tp.ag_linear(("fc1", i), ln2, self.p[p + "fc1_weight"], bias=self.p[p + "fc1_bias"],
                                      gelu_aux=pre)
         x = tp.linear_rs(act, self.p[p + "fc2_weight"], residual=x2, bias=self.p[p + "fc2_bias"], role="mlp")
-        if keep:
+        if keep and self.kept == "e4m3":
+            saved.append((K.pack(x_in), mean1, rstd1, self._keep_normed(ln1_full), K.pack(qkv), None, None,
+                          K.pack(x2), mean2, rstd2, self._keep_normed(ln2_full), K.pack(pre), None))
+        elif keep:
             saved.append((x_in, mean1, rstd1, ln1_full, qkv, attn, lse, x2, mean2, rstd2, ln2_full, pre, act))
         return x
+
+    def _norm_backward(self, name, dy, x, mean, rstd, dres, ln_ws, normed, out):
+        """Norm `name`: writes its parameter gradients; returns (dx, its gathered output
+        for the following product's weight gradient)."""
+        g, w = self.g, self.p[name + "_weight"]
+        if isinstance(x, K.Packed8):
+            again = self.p[name + "_bias"] if normed is None else None
+            dx, dw, db, y = N.layer_norm_bwd_packed(dy, x, w, mean, rstd, dres=dres, bias=again, out=out)
+            normed = y if normed is None else normed
+        else:
+            dx, dw, db = N.layer_norm_bwd(dy, x, w, mean, rstd, dres=dres, workspace=ln_ws, out=out)
+        g[name + "_weight"].copy_(dw)
+        g[name + "_bias"].copy_(db)
+        return dx, normed
 
     def _layer_backward(self, i, tape, dx, ln_ws, col_ws):
         """One transformer block backward: writes its parameter gradients and
@@ -264,6 +327,7 @@ class GPT:
         c, tp, g = self.config, self.tp, self.g
         p = f"layers.{i}."
         (x_in, mean1, rstd1, ln1_full, qkv, attn, lse, x2, mean2, rstd2, ln2_full, pre, act) = tape
+        pre, act = self._mlp_again(pre, act)
         # fc2 (row-parallel): x = x2 + RS(act @ Wfc2^T) + b
         N.column_sum(dx, out=g[p + "fc2_bias"], workspace=col_ws)
         dpre, dfull = tp.ag_linear(("fc2_bwd", i % 2), dx, self.p[p + "fc2_weight"], b_mn=True,
@@ -272,14 +336,12 @@ class GPT:
         # fc1 (column-parallel): pre = gather(ln2) @ Wfc1^T + b
         N.column_sum(dpre, out=g[p + "fc1_bias"], workspace=col_ws)
         dln2 = tp.linear_rs(dpre, self.p[p + "fc1_weight"], b_mn=True, role="mlp_bwd")
-        G.matmul(dpre, ln2_full, a_t=True, b_t=True, out=g[p + "fc1_weight"])
         M, h, W = self.M, self.h, self.world
-        dx2, dw2, db2 = N.layer_norm_bwd(dln2, x2, self.p[p + "ln2_weight"], mean2, rstd2, dres=dx,
-                                         workspace=ln_ws,
-                                         out=tp.ag_input(("attn_bwd", i % 2), M, h, h // W, dx.is_cuda))
-        g[p + "ln2_weight"].copy_(dw2)
-        g[p + "ln2_bias"].copy_(db2)
+        dx2, ln2_full = self._norm_backward(p + "ln2", dln2, x2, mean2, rstd2, dx, ln_ws, ln2_full,
+                                            tp.ag_input(("attn_bwd", i % 2), M, h, h // W, dx.is_cuda))
+        G.matmul(dpre, ln2_full, a_t=True, b_t=True, out=g[p + "fc1_weight"])
         # attention out-projection (row-parallel): x2 = x_in + RS(attn @ Wattn^T) + b
+        qkv, attn, lse = self._attention_again(qkv, attn, lse)
         N.column_sum(dx2, out=g[p + "attn_bias"], workspace=col_ws)
         dattn, dfull2 = tp.ag_linear(("attn_bwd", i % 2), dx2, self.p[p + "attn_weight"], b_mn=True)
         G.matmul(dfull2, attn, a_t=True, b_t=True, out=g[p + "attn_weight"])
@@ -287,14 +349,113 @@ class GPT:
         # QKV (column-parallel)
         N.column_sum(dqkv, out=g[p + "qkv_bias"], workspace=col_ws)
         dln1 = tp.linear_rs(dqkv, self.p[p + "qkv_weight"], b_mn=True, role="attn_bwd")
-        G.matmul(dqkv, ln1_full, a_t=True, b_t=True, out=g[p + "qkv_weight"])
         # The input gradient feeds the previous layer's FC2-backward AG->GEMM.
         nxt = tp.ag_input(("fc2_bwd", (i - 1) % 2), M, h, self.f // W, dx2.is_cuda) if i > 0 else None
-        dx, dw1, db1 = N.layer_norm_bwd(dln1, x_in, self.p[p + "ln1_weight"], mean1, rstd1, dres=dx2,
-                                        workspace=ln_ws, out=nxt)
-        g[p + "ln1_weight"].copy_(dw1)
-        g[p + "ln1_bias"].copy_(db1)
+        dx, ln1_full = self._norm_backward(p + "ln1", dln1, x_in, mean1, rstd1, dx2, ln_ws, ln1_full, nxt)
+        G.matmul(dqkv, ln1_full, a_t=True, b_t=True, out=g[p + "qkv_weight"])
         return dx
+
+    # ---------------------------------------------------------- sandwich blocks
+    def _join(self, i: int, branch: str):
+        """Parameters of the joint after layer i's branch: its norm and gate, and the
+        norm before the next branch."""
+        after = f"layers.{i}.ln2" if branch == "attn" else \
+            f"layers.{i + 1}.ln1" if i + 1 < self.config["layers"] else "final"
+        p = f"layers.{i}.{branch}_"
+        return p, after
+
+    def _join_forward(self, i, branch, x, y, site, n):
+        p, after = self._join(i, branch)
+        P = self.p
+        return N.block_join_fwd(x, y, P[p + "post_weight"], P[p + "post_bias"], P[p + "gate"],
+                                P[after + "_weight"], P[after + "_bias"], self.eps, residual_scale=self.residual_scale,
+                                out=self.tp.ag_input(site, self.M, self.h, n, x.is_cuda))
+
+    def _join_backward(self, i, branch, dh, dx, tape, normed, site, n):
+        """Gradient of a joint from that of its norm's output and of the stream; returns
+        (gradient of the stream before it, of the branch's output, the norm's output)."""
+        p, after = self._join(i, branch)
+        P, g = self.p, self.g
+        x_out, y, stats = tape
+        again = P[after + "_bias"] if normed is None else None
+        r = N.block_join_bwd(dh, dx, x_out, y, stats, P[p + "post_weight"], P[p + "post_bias"], P[p + "gate"],
+                             P[after + "_weight"], residual_scale=self.residual_scale, pre_bias=again,
+                             out=self.tp.ag_input(site, self.M, self.h, n, dh.is_cuda))
+        for name, value in ((p + "post_weight", r.dpost_weight), (p + "post_bias", r.dpost_bias),
+                            (p + "gate", r.dgate), (after + "_weight", r.dpre_weight), (after + "_bias", r.dpre_bias)):
+            g[name].copy_(value)
+        return r.dx, r.dy, r.h if normed is None else normed
+
+    def _sandwich_forward(self, x, saved, keep):
+        """All blocks; returns (the final norm's output, (x, mean, rstd, output) of the first norm)."""
+        c, tp, M, h, W = self.config, self.tp, self.M, self.h, self.world
+        ln, mean, rstd = N.layer_norm_fwd(x, self.p["layers.0.ln1_weight"], self.p["layers.0.ln1_bias"], self.eps,
+                                          out=tp.ag_input(("qkv", 0), M, h, 3 * h // W, x.is_cuda))
+        first = [self._keep(x), mean, rstd] if keep else None
+        for i in range(c["layers"]):
+            p = f"layers.{i}."
+            with tracing.scope(f"gpt.layer{i}.forward"):
+                qkv, ln1_full = tp.ag_linear(("qkv", i), ln, self.p[p + "qkv_weight"], bias=self.p[p + "qkv_bias"])
+                attn, lse = A.forward(qkv, c["micro_batch"], c["sequence"], self.lh)
+                y1 = tp.linear_rs(attn, self.p[p + "attn_weight"], bias=self.p[p + "attn_bias"], role="attn")
+                x2, ln, st1 = self._join_forward(i, "attn", x, y1, ("fc1", i), self.f // W)
+                pre = torch.empty((M, self.f // W), dtype=torch.bfloat16, device=self.device)
+                act, ln2_full = tp.ag_linear(("fc1", i), ln, self.p[p + "fc1_weight"], bias=self.p[p + "fc1_bias"],
+                                             gelu_aux=pre)
+                y2 = tp.linear_rs(act, self.p[p + "fc2_weight"], bias=self.p[p + "fc2_bias"], role="mlp")
+                last = i + 1 == c["layers"]
+                x, ln, st2 = self._join_forward(i, "mlp", x2, y2, ("head", 0) if last else ("qkv", i + 1),
+                                                self.Vl if last else 3 * h // W)
+                if keep:
+                    packed = self.kept == "e4m3"
+                    saved.append((self._keep_normed(ln1_full), self._keep(qkv), None if packed else attn,
+                                  None if packed else lse, (self._keep(x2), self._keep(y1), st1),
+                                  self._keep_normed(ln2_full), self._keep(pre), None if packed else act,
+                                  (self._keep(x), self._keep(y2), st2)))
+        return ln, first
+
+    def _sandwich_backward(self, dlnf, saved, first, lnf_full, ln_ws, col_ws):
+        c, tp, g = self.config, self.tp, self.g
+        M, h, W, L = self.M, self.h, self.world, self.config["layers"]
+        dx, dy, _ = self._join_backward(L - 1, "mlp", dlnf, None, saved[L - 1][8], lnf_full,
+                                        ("fc2_bwd", (L - 1) % 2), self.f // W)
+        for i in reversed(range(L)):
+            p = f"layers.{i}."
+            with tracing.scope(f"gpt.layer{i}.backward"):
+                ln1_full, qkv, attn, lse, join1, ln2_full, pre, act, _ = saved[i]
+                pre, act = self._mlp_again(pre, act)
+                N.column_sum(dy, out=g[p + "fc2_bias"], workspace=col_ws)
+                dpre, dfull = tp.ag_linear(("fc2_bwd", i % 2), dy, self.p[p + "fc2_weight"], b_mn=True,
+                                           gelu_grad_of=pre)
+                G.matmul(dfull, act, a_t=True, b_t=True, out=g[p + "fc2_weight"])
+                N.column_sum(dpre, out=g[p + "fc1_bias"], workspace=col_ws)
+                dln = tp.linear_rs(dpre, self.p[p + "fc1_weight"], b_mn=True, role="mlp_bwd")
+                dx, dy, ln2_full = self._join_backward(i, "attn", dln, dx, join1, ln2_full, ("attn_bwd", i % 2), h // W)
+                G.matmul(dpre, ln2_full, a_t=True, b_t=True, out=g[p + "fc1_weight"])
+                qkv, attn, lse = self._attention_again(qkv, attn, lse)
+                N.column_sum(dy, out=g[p + "attn_bias"], workspace=col_ws)
+                dattn, dfull = tp.ag_linear(("attn_bwd", i % 2), dy, self.p[p + "attn_weight"], b_mn=True)
+                G.matmul(dfull, attn, a_t=True, b_t=True, out=g[p + "attn_weight"])
+                dqkv = A.backward(qkv, attn, dattn, lse, c["micro_batch"], c["sequence"], self.lh)
+                N.column_sum(dqkv, out=g[p + "qkv_bias"], workspace=col_ws)
+                dln = tp.linear_rs(dqkv, self.p[p + "qkv_weight"], b_mn=True, role="attn_bwd")
+                if i:
+                    dx, dy, ln1_full = self._join_backward(i - 1, "mlp", dln, dx, saved[i - 1][8], ln1_full,
+                                                           ("fc2_bwd", (i - 1) % 2), self.f // W)
+                else:
+                    dx, ln1_full = self._norm_backward("layers.0.ln1", dln, *first, dx, ln_ws, ln1_full, None)
+                G.matmul(dqkv, ln1_full, a_t=True, b_t=True, out=g[p + "qkv_weight"])
+        return dx
+
+    # ------------------------------------------------------------------ scoring
+    @torch.no_grad()
+    def score(self, tokens, targets, top_k: int = 0) -> CE.TokenScores:
+        """Log probability of each target, entropy and the `top_k` most probable tokens
+        of every position of one micro-batch (forward only; a negative target is not
+        scored).  The same on every rank."""
+        logits, _ = self._logits(tokens, targets, keep=False)
+        scores, _ = CE.token_logprobs(logits, targets, top_k, self.tp.group, self.rank, self.world)
+        return scores
 
     @torch.no_grad()
     def loss(self, tokens, targets) -> torch.Tensor:
@@ -304,16 +465,37 @@ class GPT:
 
     # ------------------------------------------------------------ backward
     @torch.no_grad()
-    def forward_backward(self, tokens, targets, loss_scale: float = 1.0) -> torch.Tensor:
+    def forward_backward(self, tokens, targets, loss_scale: float = 1.0, weights: torch.Tensor | None = None,
+                         entropy_bonus: float = 0.0) -> torch.Tensor:
         """Forward + backward of one micro-batch; gradients of `loss * loss_scale`
-        are written into `self.store.grad`.  Returns the (unscaled) mean loss."""
-        loss, tape = self._forward(tokens, targets, keep=True, loss_scale=1.0)
-        self._backward(tape, loss_scale)
+        are written into `self.store.grad`.  Returns the (unscaled) mean loss.
+
+        The loss is the mean cross-entropy; with `weights` (FP32, one a position) or an
+        `entropy_bonus` it is -mean(weight * log p(target) + entropy_bonus * entropy) over
+        the positions, of which those with a negative target count as zero."""
+        if weights is None and entropy_bonus == 0.0:
+            loss, tape = self._forward(tokens, targets, keep=True, loss_scale=1.0)
+            self._backward(tape, loss_scale)
+            return loss
+        if weights is not None and (weights.shape != targets.shape or weights.dtype != torch.float32):
+            raise ValueError("weights must be FP32, one for each target")
+        logits, trunk = self._logits(tokens, targets, keep=True)
+        scores, state = CE.token_logprobs(logits, targets, 0, self.tp.group, self.rank, self.world)
+        scored = (targets >= 0).float()
+        w = scored if weights is None else weights * scored
+        bonus = scored * entropy_bonus
+        loss = -((w * scores.logprob).sum() + (bonus * scores.entropy).sum()).reshape(1) / self.M
+        scale = -loss_scale / self.M
+        CE.token_logprobs_backward(logits, targets, state, w * scale, bonus * scale, out=logits)
+        self._backward((tokens, targets, trunk, logits, None), loss_scale)
         return loss
 
     def _backward(self, tape, loss_scale: float):
+        """Gradients of every parameter.  Without a cross-entropy state in the tape, the
+        logits hold their own gradient already."""
         c, tp = self.config, self.tp
-        tokens, targets, saved, x_final, meanf, rstdf, lnf_full, logits, ce_state = tape
+        tokens, targets, trunk, logits, ce_state = tape
+        saved, x_final, meanf, rstdf, lnf_full = trunk
         M = self.M
         start = self.rank * self.Vl
         g = self.g
@@ -321,9 +503,14 @@ class GPT:
         col_ws = self._workspace("col", 64 * max(self.f // self.world, 3 * self.h // self.world, self.h),
                                  torch.float32)
         # Cross-entropy -> dlogits (in place), LM head (tied embedding)
-        CE.backward(logits, targets, ce_state, loss_scale / M)
+        if ce_state is not None:
+            CE.backward(logits, targets, ce_state, loss_scale / M)
         dlnf = tp.linear_rs(logits, self.p["embedding"], b_mn=True, role="head")
         G.matmul(logits, lnf_full, a_t=True, b_t=True, out=g["embedding"])
+        if self.sandwich:
+            dx = self._sandwich_backward(dlnf, saved, x_final, lnf_full, ln_ws, col_ws)
+            self._embedding_backward(tokens, dx, start)
+            return
         L = c["layers"]
         dx, dwf, dbf = N.layer_norm_bwd(dlnf, x_final, self.p["final_weight"], meanf, rstdf, workspace=ln_ws,
                                         out=tp.ag_input(("fc2_bwd", (L - 1) % 2), M, self.h, self.f // self.world,
@@ -333,10 +520,13 @@ class GPT:
         for i in reversed(range(c["layers"])):
             with tracing.scope(f"gpt.layer{i}.backward"):
                 dx = self._layer_backward(i, saved[i], dx, ln_ws, col_ws)
+        self._embedding_backward(tokens, dx, start)
+
+    def _embedding_backward(self, tokens, dx, start):
         # value = scatter_sum(embedding contributions) + position
-        E.position_grad(dx, c["sequence"], self.rank * self.Ml, out=g["position"])
-        dcontrib = tp.gather_rows(dx)
-        E.lookup_grad(tokens, dcontrib, g["embedding"], start, accumulate=True)
+        E.position_grad(dx, self.config["sequence"], self.rank * self.Ml, out=self.g["position"])
+        dcontrib = self.tp.gather_rows(dx)
+        E.lookup_grad(tokens, dcontrib, self.g["embedding"], start, accumulate=True)
 
     def close(self):
         self.tp.close()

@@ -26,7 +26,8 @@ from ..utils import tracing
 
 class Trainer:
     def __init__(self, model: GPT, *, lr: float | None = None, weight_decay: float | None = None,
-                 betas=(0.9, 0.95), eps: float = 1e-8, max_grad_norm: float | None = None):
+                 betas=(0.9, 0.95), eps: float = 1e-8, max_grad_norm: float | None = None,
+                 entropy_bonus: float = 0.0):
         c = model.config
         self.model = model
         self.lr = c["learning_rate"] if lr is None else lr
@@ -34,6 +35,7 @@ class Trainer:
         self.max_grad_norm = c["max_grad_norm"] if max_grad_norm is None else max_grad_norm
         self.beta1, self.beta2 = betas
         self.eps = eps
+        self.entropy_bonus = entropy_bonus
         st = model.store
         self.master = st.flat.float()
         self.m = torch.zeros_like(self.master)
@@ -46,15 +48,17 @@ class Trainer:
         self.step_count = 0
 
     def step(self, batches):
-        """One optimizer step over `batches` = [(tokens, labels)] * accumulation_steps.
+        """One optimizer step over `batches` = [(tokens, labels)] * accumulation_steps, or
+        [(tokens, labels, weights)] for the weighted loss of `GPT.forward_backward`.
         Returns device tensors (mean loss, squared global grad norm)."""
         model, st = self.model, self.model.store
         if len(batches) != self.acc:
             raise ValueError(f"expected {self.acc} micro-batches")
         self.loss_sum.zero_()
-        for mb, (tokens, labels) in enumerate(batches):
+        for mb, (tokens, labels, *weights) in enumerate(batches):
             with tracing.scope(f"trainer.micro_batch{mb}"):
-                loss = model.forward_backward(tokens, labels, loss_scale=1.0 / self.acc)
+                loss = model.forward_backward(tokens, labels, 1.0 / self.acc, *weights,
+                                              entropy_bonus=self.entropy_bonus)
                 self.loss_sum.add_(loss.reshape(()) / self.acc)
                 if self.grad32 is not None:
                     self.grad32.add_(st.grad)
@@ -90,11 +94,11 @@ class Trainer:
             self.grad32.zero_()
 
     def train_step(self, host_batches):
-        """Public one-call step: copies each micro-batch's (tokens, labels) from
-        (pinned) host memory to the device, runs `step`, and returns host floats
+        """Public one-call step: copies each micro-batch's (tokens, labels[, weights])
+        from (pinned) host memory to the device, runs `step`, and returns host floats
         (mean loss, global grad norm)."""
         dev = self.model.device
-        batches = [(t.to(dev, non_blocking=True), l.to(dev, non_blocking=True)) for t, l in host_batches]
+        batches = [tuple(t.to(dev, non_blocking=True) for t in batch) for batch in host_batches]
         return self.step_host(batches)
 
     def step_host(self, batches):
