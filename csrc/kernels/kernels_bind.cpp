@@ -232,7 +232,7 @@ void need_rows(const at::Tensor& t, const at::Tensor& like, int64_t rows, int64_
 }
 void need_vector(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
   need_like(t, like, like.scalar_type(), name);
-  TORCH_CHECK(t.numel() == n, name, " must hold ", std::to_string(n), " values");
+  TORCH_CHECK(t.dim() == 1 && t.numel() == n, name, " must hold ", std::to_string(n), " values");
 }
 void need_floats(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
   need_like(t, like, at::kFloat, name);
@@ -247,7 +247,7 @@ void score_fwd(const at::Tensor& logits, const at::Tensor& targets, int64_t star
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   need_rows(logits, logits, rows, vocab, "logits");
   need_like(targets, logits, at::kLong, "targets");
-  TORCH_CHECK(targets.numel() == rows, "targets must hold one id a row");
+  TORCH_CHECK(targets.dim() == 1 && targets.numel() == rows, "targets must hold one id a row");
   float* f = nullptr;
   int64_t* ids = nullptr;
   float* rec = nullptr;
@@ -289,7 +289,7 @@ void score_bwd(const at::Tensor& logits, const at::Tensor& targets, int64_t star
   need_rows(logits, logits, rows, vocab, "logits");
   need_rows(out, logits, rows, vocab, "out");
   need_like(targets, logits, at::kLong, "targets");
-  TORCH_CHECK(targets.numel() == rows, "targets must hold one id a row");
+  TORCH_CHECK(targets.dim() == 1 && targets.numel() == rows, "targets must hold one id a row");
   need_floats(state, logits, 3 * rows, "state");
   need_floats(dlogprob, logits, rows, "dlogprob");
   if (dentropy) need_floats(*dentropy, logits, rows, "dentropy");
@@ -411,6 +411,121 @@ void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const a
   const c10::cuda::CUDAGuard g(dh.device());
   ok(k::join_bwd(c, cur()), branch ? "block_join_bwd" : "layer_norm_bwd_packed");
 }
+
+// The operators' public forms: outputs are allocated here, so that a call costs one
+// crossing from Python.  Arguments are checked by the functions above.
+at::Tensor rows_like(const at::Tensor& t) { return at::empty({t.size(0), t.size(1)}, t.options()); }
+void need_matrix(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2, name, " must be a matrix on CUDA");
+}
+void need_own_rows(const c10::optional<at::Tensor>& t, const char* name) {
+  if (t) TORCH_CHECK(t->dim() == 2 && (t->size(0) < 2 || t->stride(0) >= t->size(1)), name, " needs rows of its own");
+}
+using Tensors = std::vector<c10::optional<at::Tensor>>;
+
+Tensors token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k) {
+  need_matrix(logits, "logits");
+  TORCH_CHECK(top_k >= 0 && top_k <= 32, "top_k is out of range");
+  const int64_t rows = logits.size(0);
+  at::Tensor out = at::empty({rows * (5 + top_k)}, logits.options().dtype(at::kFloat));
+  at::Tensor ids = at::empty({rows, top_k}, logits.options().dtype(at::kLong));
+  if (rows) score_fwd(logits, targets.contiguous(), 0, logits.size(1), top_k, out, ids, c10::nullopt);
+  return {out.narrow(0, 0, rows), out.narrow(0, rows, rows), out.narrow(0, 5 * rows, rows * top_k).view({rows, top_k}),
+          ids, out.narrow(0, 2 * rows, 3 * rows).view({3, rows})};
+}
+at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& targets, int64_t start,
+                                   int64_t vocab_total, const at::Tensor& state, const at::Tensor& dlogprob,
+                                   const c10::optional<at::Tensor>& dentropy, const c10::optional<at::Tensor>& out) {
+  need_matrix(logits, "logits");
+  need_own_rows(out, "out");
+  const int64_t rows = logits.size(0);
+  TORCH_CHECK(state.dim() == 2 && state.size(0) == 3 && state.size(1) == rows, "the state belongs to other logits");
+  TORCH_CHECK(dlogprob.dim() == 1 && dlogprob.numel() == rows, "dlogprob must hold one value a row");
+  TORCH_CHECK(!dentropy || (dentropy->dim() == 1 && dentropy->numel() == rows), "dentropy must hold one value a row");
+  at::Tensor to = out ? *out : rows_like(logits);
+  if (rows) {
+    c10::optional<at::Tensor> de;
+    if (dentropy) de = dentropy->contiguous();
+    score_bwd(logits, targets.contiguous(), start, vocab_total, state, dlogprob.contiguous(), de, to);
+  }
+  return to;
+}
+at::Tensor pack(const at::Tensor& x) {
+  need_matrix(x, "x");
+  at::Tensor data = at::empty({x.size(0), k::act_pack_row_bytes(x.size(1))}, x.options().dtype(at::kByte));
+  if (x.size(0)) act_pack(x, data);
+  return data;
+}
+Tensors unpack(const at::Tensor& data, int64_t cols, bool fp32, bool gelu) {
+  at::Tensor out = at::empty({data.size(0), cols}, data.options().dtype(fp32 ? at::kFloat : at::kBFloat16));
+  c10::optional<at::Tensor> act;
+  if (gelu) act = at::empty_like(out);
+  if (out.numel()) act_unpack(data, out, act);
+  return {out, act};
+}
+Tensors block_join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tensor& pw, const at::Tensor& pb,
+                       const at::Tensor& gate, const at::Tensor& w, const at::Tensor& b, double alpha, double eps,
+                       const c10::optional<at::Tensor>& out) {
+  need_matrix(x, "x");
+  need_own_rows(out, "out");
+  at::Tensor u = rows_like(x);
+  at::Tensor h = out ? *out : rows_like(x);
+  at::Tensor stats = at::empty({4, x.size(0)}, x.options().dtype(at::kFloat));
+  if (x.size(0)) join_fwd(x, y, pw, pb, gate, w, b, u, h, stats, alpha, eps);
+  return {u, h, stats};
+}
+struct Spare {  // gradients of the parameters, and a workspace that is large enough
+  at::Tensor grads, workspace;
+  Spare(const at::Tensor& dh, bool branch, const c10::optional<at::Tensor>& given) {
+    const int64_t rows = dh.size(0), cols = dh.size(1);
+    TORCH_CHECK(cols > 0 && cols <= k::join_max_cols(), "the hidden size is out of range");
+    grads = at::empty({branch ? 5 : 2, cols}, dh.options());
+    if (!rows) {
+      grads.zero_();
+      return;
+    }
+    const int64_t size = join_bwd_workspace(rows, cols, branch);
+    workspace = given && given->numel() >= size ? *given : at::empty({size}, dh.options().dtype(at::kFloat));
+  }
+};
+// (dx, dy, dpost_weight, dpost_bias, dgate, dpre_weight, dpre_bias, h)
+Tensors block_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const at::Tensor& u,
+                       const at::Tensor& y, const at::Tensor& stats, const at::Tensor& pw, const at::Tensor& pb,
+                       const at::Tensor& gate, const at::Tensor& w, const c10::optional<at::Tensor>& b,
+                       const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& workspace, double alpha) {
+  need_matrix(dh, "dh");
+  need_own_rows(out, "out");
+  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == 4 && stats.size(1) == dh.size(0) && stats.is_contiguous(),
+              "stats must be contiguous [4, rows]");
+  TORCH_CHECK(u.scalar_type() == y.scalar_type(), "x_out and y are kept in the same form");
+  Spare spare(dh, true, workspace);
+  at::Tensor dx = rows_like(dh);
+  c10::optional<at::Tensor> dy = out ? *out : rows_like(dh), h;
+  if (b) h = rows_like(dh);
+  if (dh.size(0))
+    join_bwd(dh, du, u, y, stats.select(0, 2), stats.select(0, 3), stats.select(0, 0), stats.select(0, 1), pw, pb,
+             gate, w, b, dx, dy, h, spare.grads, spare.workspace, alpha);
+  const at::Tensor& g = spare.grads;
+  return {dx, dy, g.select(0, 2), g.select(0, 3), g.select(0, 4), g.select(0, 0), g.select(0, 1), h};
+}
+// (dx, dweight, dbias, y)
+Tensors layer_norm_bwd_packed(const at::Tensor& dy, const c10::optional<at::Tensor>& dres, const at::Tensor& x,
+                              const at::Tensor& mean, const at::Tensor& rstd, const at::Tensor& w,
+                              const c10::optional<at::Tensor>& b, const c10::optional<at::Tensor>& out,
+                              const c10::optional<at::Tensor>& workspace) {
+  need_matrix(dy, "dy");
+  need_own_rows(out, "out");
+  TORCH_CHECK(mean.dim() == 1 && rstd.dim() == 1 && mean.numel() == dy.size(0) && rstd.numel() == dy.size(0),
+              "mean and rstd must hold one value a row");
+  Spare spare(dy, false, workspace);
+  at::Tensor dx = out ? *out : rows_like(dy);
+  c10::optional<at::Tensor> y, none;
+  if (b) y = rows_like(dy);
+  if (dy.size(0))
+    join_bwd(dy, dres, x, none, mean, rstd, none, none, none, none, none, w, b, dx, none, y, spare.grads,
+             spare.workspace, 1.0);
+  return {dx, spare.grads.select(0, 0), spare.grads.select(0, 1), y};
+}
 }  // namespace
 
 // Launch entry points touch no Python object: the GIL is released while they
@@ -435,6 +550,13 @@ void register_kernels(pybind11::module& m) {
   m.def("score_fwd", &score_fwd, nogil());
   m.def("score_merge", &score_merge, nogil());
   m.def("score_bwd", &score_bwd, nogil());
+  m.def("token_logprobs", &token_logprobs, nogil());
+  m.def("token_logprobs_backward", &token_logprobs_backward, nogil());
+  m.def("pack", &pack, nogil());
+  m.def("unpack", &unpack, nogil());
+  m.def("block_join_fwd", &block_join_fwd, nogil());
+  m.def("block_join_bwd", &block_join_bwd, nogil());
+  m.def("layer_norm_bwd_packed", &layer_norm_bwd_packed, nogil());
   m.def("act_pack_row_bytes", &k::act_pack_row_bytes);
   m.def("act_pack", &act_pack, nogil());
   m.def("act_unpack", &act_unpack, nogil());

@@ -148,29 +148,25 @@ struct Vec {  // one 16-byte load
   }
 };
 
-// One thread's running state.
+// One thread's sums over its part of a row, by the definitions: any values, with
+// infinities and NaN.  Rows of ordinary values take `Fast` below.
 template <bool TOP>
 struct Running {
   Sums a{-INFINITY, 0.f, 0.f};
   unsigned best = 0, best_at = 0xffffffffu;  // order_of the largest value, start of its vector
 
-  // N values of a chunk; every COUNT of them begin at index at[i / COUNT].
-  template <int N, int COUNT>
-  __device__ __forceinline__ void add(const float* v, const unsigned* at) {
-    float top = -INFINITY;
+  // N values that begin at index `at`.
+  template <int N>
+  __device__ __forceinline__ void add(const float* v, unsigned at) {
+    float top = v[0];
 #pragma unroll
-    for (int g = 0; g < N / COUNT; ++g) {
-      float t = v[g * COUNT];
-#pragma unroll
-      for (int i = 1; i < COUNT; ++i) t = max_nan(t, v[g * COUNT + i]);
-      if (TOP) {
-        const unsigned o = order_of(t);
-        if (o > best) {
-          best = o;
-          best_at = at[g];
-        }
+    for (int i = 1; i < N; ++i) top = max_nan(top, v[i]);
+    if (TOP) {
+      const unsigned o = order_of(top);
+      if (o > best) {
+        best = o;
+        best_at = at;
       }
-      top = max_nan(top, t);
     }
     const float m = max_nan(a.m, top);
     const float base = m == -INFINITY ? 0.f : m;
@@ -189,6 +185,144 @@ struct Running {
   }
   __device__ __forceinline__ Key key() const { return best ? Key(best) << 32 | Key(~best_at) : 0; }
 };
+
+// The same for rows whose largest value lies within +-kPlain, in half the
+// instructions: t = z log2 e - R <= 0 with one fused multiply-add, R = fl(m log2 e) the
+// running reference, two elements an instruction (f32x2), the maximum of 16-bit
+// types on packed pairs.  Values below -kFloor (-inf above all) are lifted to it,
+// which leaves 2^t zero and t finite.  R is a function of m, so sums join without
+// further state, and its rounding is taken out once per row (`natural`).
+constexpr float kFloor = 1e30f, kPlain = 1e29f;
+template <typename T> struct Packed2;
+template <> struct Packed2<__nv_bfloat16> {
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+  static __device__ __forceinline__ unsigned floor() { return 0xf149f149u; }  // -0.995e30
+  static __device__ __forceinline__ Two floats(unsigned w) {
+    return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+template <> struct Packed2<__half> {
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const unsigned*>(&r);
+  }
+  static __device__ __forceinline__ unsigned floor() { return 0xfbfffbffu; }  // -65504, the type's lowest
+  static __device__ __forceinline__ Two floats(unsigned w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return two(f.x, f.y);
+  }
+};
+// Largest value and the values lifted to the floor of one 16-byte vector.
+template <typename T>
+struct Loaded {
+  static constexpr int kPairs = 8 / int(sizeof(T) / 2) / 2;
+  static __device__ __forceinline__ void read(const uint4& raw, float& top, Two* z) {
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+    using P = Packed2<T>;
+    unsigned t = P::larger(P::larger(w[0], w[1]), P::larger(w[2], w[3]));
+    t = P::larger(t, t >> 16 | t << 16);
+    top = both(P::floats(t)).x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = P::floats(P::larger(w[i], P::floor()));
+  }
+};
+template <>
+struct Loaded<float> {
+  static constexpr int kPairs = 2;
+  static __device__ __forceinline__ void read(const uint4& raw, float& top, Two* z) {
+    const float v[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z), __uint_as_float(raw.w)};
+    top = max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) z[i] = two(fmaxf(v[2 * i], -kFloor), fmaxf(v[2 * i + 1], -kFloor));
+  }
+};
+// Where the running maximum begins: at or above every lifted value, so that t <= 0,
+// and so low that what was counted there vanishes in a row whose largest value is
+// above `plain_low` (FP16's floor is no lower than its lowest number).
+template <typename T> __device__ __forceinline__ float start_low() { return -9.9e29f; }
+template <> __device__ __forceinline__ float start_low<__half>() { return -65504.f; }
+template <typename T> __device__ __forceinline__ float plain_low() { return -kPlain; }
+template <> __device__ __forceinline__ float plain_low<__half>() { return -6e4f; }
+
+// R: rounded on its own everywhere (a product contracted into a following
+// difference would be another reference).
+__device__ __forceinline__ float reference(float m) { return __fmul_rn(m, kLog2e); }
+
+template <typename T, bool TOP>
+struct Fast {
+  float m = start_low<T>(), best = -INFINITY;
+  unsigned best_at = 0xffffffffu;
+  Two s = 0, u = 0;  // of even and odd elements
+
+  __device__ __forceinline__ void raise(float top) {
+    const float next = max_nan(m, top);
+    const float d = reference(m) - reference(next);
+    const float f = fast_exp2(d);
+    u = two_mul(two_fma(two(d, d), s, u), two(f, f));
+    s = two_mul(s, two(f, f));
+    m = next;
+  }
+  __device__ __forceinline__ void count(Two z, Two scale, Two minus_r) {
+    const Two t = two_fma(z, scale, minus_r);
+    const float2 f = both(t);
+    const Two e = two(fast_exp2(f.x), fast_exp2(f.y));
+    s = two_add(s, e);
+    u = two_fma(e, t, u);
+  }
+  // COUNT vectors; `at` is the first one's index and `step` the distance to the next.
+  template <int COUNT>
+  __device__ __forceinline__ void add(const uint4* raw, unsigned at, unsigned step) {
+    constexpr int P = Loaded<T>::kPairs;
+    Two z[COUNT * P];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      float t;
+      Loaded<T>::read(raw[i], t, z + i * P);
+      if (TOP && t > best) {
+        best = t;
+        best_at = at + i * step;
+      }
+      top = max_nan(top, t);
+    }
+    raise(top);
+    const float r = -reference(m);
+    const Two scale = two(kLog2e, kLog2e), minus_r = two(r, r);
+#pragma unroll
+    for (int i = 0; i < COUNT * P; ++i) count(z[i], scale, minus_r);
+  }
+  __device__ __forceinline__ void add_one(float v, unsigned at) {
+    if (TOP && v > best) {
+      best = v;
+      best_at = at;
+    }
+    raise(v);
+    const float t = fmaf(fmaxf(v, -kFloor), kLog2e, -reference(m));
+    const float e = fast_exp2(t);
+    s = two_add(s, two(e, 0.f));
+    u = two_fma(two(e, 0.f), two(t, 0.f), u);
+  }
+  __device__ __forceinline__ Key key() const { return best_at != 0xffffffffu ? make_key(best, best_at) : 0; }
+  // The warp's sums relative to its own maximum, in every lane.
+  __device__ __forceinline__ Sums warp_total() const {
+    float top = m;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(kAllLanes, top, d));
+    const float2 ss = both(s), uu = both(u);
+    const float d = reference(m) - reference(top), f = fast_exp2(d);
+    const float sum = ss.x + ss.y;
+    return Sums{top, warp_sum(sum * f), warp_sum((uu.x + uu.y + d * sum) * f)};
+  }
+};
+// From the reference fl(m log2 e) and log2 units to sums of e^(z - m).
+__device__ __forceinline__ Sums natural(Sums a) {
+  const float off = fmaf(a.m, kLog2e, -reference(a.m));
+  const float f = fast_exp2(-off);
+  return Sums{a.m, a.s * f, (a.u - off * a.s) * f * 0.69314718055994530942f};
+}
 
 // The part of a row that one CTA reads: `head` single values up to a 16-byte
 // boundary, `vectors` vectors, `tail` single values.
@@ -322,64 +456,92 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_
   const Part<T> part(x, begin, end);
   constexpr int kN = Vec<T>::kN;
 
-  Running<TOP> run;
-  if (unsigned(tid) < part.head) {
-    const float v = to_float(part.x[tid]);
-    const unsigned at = part.lo + tid;
-    run.template add<1, 1>(&v, &at);
-  }
-  unsigned j = tid;
-  for (; j + (kUnroll - 1) * kThreads < part.vectors; j += kUnroll * kThreads) {
-    Vec<T> vec[kUnroll];
-    float v[kUnroll * kN];
-    unsigned at[kUnroll];
+  // Sums of the CTA's part: by the fast form, or by the definitions where the
+  // largest value says that the fast one does not hold.
+  Key key = 0;
+  {
+    Fast<T, TOP> run;
+    if (unsigned(tid) < part.head) run.add_one(to_float(part.x[tid]), part.lo + tid);
+    const uint4* vectors = reinterpret_cast<const uint4*>(part.x + part.head);
+    unsigned j = tid;
+    for (; j + (kUnroll - 1) * kThreads < part.vectors; j += kUnroll * kThreads) {
+      uint4 raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) vec[i].load(part.x + part.vector_at(j + i * kThreads));
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      vec[i].get(v + i * kN);
-      at[i] = part.lo + part.vector_at(j + i * kThreads);
+      for (int i = 0; i < kUnroll; ++i) raw[i] = vectors[j + i * kThreads];
+      run.template add<kUnroll>(raw, part.lo + part.vector_at(j), kThreads * kN);
     }
-    run.template add<kUnroll * kN, kN>(v, at);
+    for (; j < part.vectors; j += kThreads) {
+      const uint4 raw = vectors[j];
+      run.template add<1>(&raw, part.lo + part.vector_at(j), 0);
+    }
+    if (unsigned(tid) < part.tail) {
+      const unsigned i = part.vector_at(part.vectors) + tid;
+      run.add_one(to_float(part.x[i]), part.lo + i);
+    }
+    const Sums a = run.warp_total();
+    if (TOP) key = run.key();
+    if (lane == 0) warp_sums[warp] = a;
   }
-  for (; j < part.vectors; j += kThreads) {
-    Vec<T> vec;
-    float v[kN];
-    const unsigned at = part.lo + part.vector_at(j);
-    vec.load(part.x + part.vector_at(j));
-    vec.get(v);
-    run.template add<kN, kN>(v, &at);
-  }
-  if (unsigned(tid) < part.tail) {
-    const unsigned i = part.vector_at(part.vectors) + tid;
-    const float v = to_float(part.x[i]);
-    const unsigned at = part.lo + i;
-    run.template add<1, 1>(&v, &at);
-  }
-
-  Sums a = run.a;
+  __syncthreads();
+  float top = warp_sums[0].m;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    Sums b;
-    b.m = __shfl_xor_sync(kAllLanes, a.m, d);
-    b.s = __shfl_xor_sync(kAllLanes, a.s, d);
-    b.u = __shfl_xor_sync(kAllLanes, a.u, d);
-    // The lower lane's sums come first on both sides, so both get the same bits.
-    a = lane & d ? join(b, a) : join(a, b);
-  }
-  if (lane == 0) warp_sums[warp] = a;
-  if constexpr (TOP) block_top(part, run.key(), o.k, sh);  // synchronises
-  else __syncthreads();
-  if (tid == 0) {
-    a = warp_sums[0];
+  for (int w = 1; w < kWarps; ++w) top = max_nan(top, warp_sums[w].m);
+  const bool plain = top > plain_low<T>() && top < kPlain;
+  if (plain) {
+    if (tid == 0) {
+      Sums a{top, 0.f, 0.f};
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) a = join(a, warp_sums[w]);
-    block_sums = a;
+      for (int w = 0; w < kWarps; ++w) {
+        const float d = reference(warp_sums[w].m) - reference(top), f = fast_exp2(d);
+        a.s += warp_sums[w].s * f;
+        a.u += (warp_sums[w].u + d * warp_sums[w].s) * f;
+      }
+      block_sums = natural(a);
+    }
+  } else {
+    Running<TOP> run;
+    if (unsigned(tid) < part.head) {
+      const float v = to_float(part.x[tid]);
+      run.template add<1>(&v, part.lo + tid);
+    }
+    for (unsigned j = tid; j < part.vectors; j += kThreads) {
+      Vec<T> vec;
+      float v[kN];
+      vec.load(part.x + part.vector_at(j));
+      vec.get(v);
+      run.template add<kN>(v, part.lo + part.vector_at(j));
+    }
+    if (unsigned(tid) < part.tail) {
+      const unsigned i = part.vector_at(part.vectors) + tid;
+      const float v = to_float(part.x[i]);
+      run.template add<1>(&v, part.lo + i);
+    }
+    Sums a = run.a;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      Sums b;
+      b.m = __shfl_xor_sync(kAllLanes, a.m, d);
+      b.s = __shfl_xor_sync(kAllLanes, a.s, d);
+      b.u = __shfl_xor_sync(kAllLanes, a.u, d);
+      // The lower lane's sums come first on both sides, so both get the same bits.
+      a = lane & d ? join(b, a) : join(a, b);
+    }
+    __syncthreads();  // every thread has read the fast form's maxima
+    if (lane == 0) warp_sums[warp] = a;
+    __syncthreads();
+    if (tid == 0) {
+      a = warp_sums[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) a = join(a, warp_sums[w]);
+      block_sums = a;
+    }
+    if (TOP) key = run.key();
   }
+  if constexpr (TOP) block_top(part, key, o.k, sh);  // synchronises
   if (C > 1) cluster.sync();
   else __syncthreads();
   if (rank == 0 && warp == 0) {
-    a = block_sums;
+    Sums a = block_sums;
     for (unsigned r = 1; r < C; ++r) a = join(a, *cluster.map_shared_rank(&block_sums, r));
     Key list = 0;
     if constexpr (TOP) {

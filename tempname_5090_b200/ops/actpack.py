@@ -50,6 +50,13 @@ class Packed8:
             raise ValueError("packed data must start on a 16-byte boundary")
         self.data, self.cols, self.dtype = data, cols, dtype
 
+    @classmethod
+    def _of(cls, data, cols, dtype):
+        """`pack`'s own result, which needs no checks."""
+        p = cls.__new__(cls)
+        p.data, p.cols, p.dtype = data, cols, dtype
+        return p
+
     @property
     def shape(self):
         return torch.Size((self.data.shape[0], self.cols))
@@ -68,19 +75,30 @@ class Packed8:
 
 def pack(x: torch.Tensor) -> Packed8:
     """Keep x [rows, cols] (BF16 or FP32, any row stride) in 8 bits."""
+    if x.is_cuda:
+        try:
+            data = lib().pack(x)
+        except (RuntimeError, TypeError):
+            _check_packable(x)
+            raise
+        count_launch()
+        return Packed8._of(data, x.shape[1], x.dtype)
+    _check_packable(x)
+    return _pack_cpu(x)
+
+
+def _check_packable(x):
     if x.dim() != 2 or x.dtype not in DTYPES:
         raise ValueError("pack takes a BF16 or FP32 matrix")
-    rows, cols = x.shape
-    if cols == 0:
+    if x.shape[1] == 0:
         raise ValueError("pack needs at least one column")
-    if cols > 1 and x.stride(1) != 1:
+    if x.shape[1] > 1 and x.stride(1) != 1:
         raise ValueError("pack needs contiguous rows")
-    if x.is_cuda:
-        data = torch.empty((rows, row_bytes(cols)), dtype=torch.uint8, device=x.device)
-        if rows:
-            lib().act_pack(x, data)
-            count_launch()
-        return Packed8(data, cols, x.dtype)
+
+
+@torch.no_grad()
+def _pack_cpu(x):
+    rows, cols = x.shape
     if not rows:
         return Packed8(torch.empty((0, row_bytes(cols)), dtype=torch.uint8), cols, x.dtype)
     groups = torch.nn.functional.pad(x.float(), (0, -cols % GROUP)).view(rows, -1, GROUP)
@@ -114,11 +132,8 @@ def unpack(p: Packed8) -> torch.Tensor:
     """The kept values, [rows, cols] of p.dtype."""
     _check(p)
     if p.is_cuda:
-        out = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-        if out.numel():
-            lib().act_unpack(p.data, out, None)
-            count_launch()
-        return out
+        count_launch()
+        return lib().unpack(p.data, p.cols, p.dtype == torch.float32, False)[0]
     return _values(p).to(p.dtype)
 
 
@@ -126,11 +141,8 @@ def unpack_gelu(p: Packed8):
     """(x, GeLU(x)) of the kept pre-activation x, both [rows, cols] of p.dtype."""
     _check(p)
     if p.is_cuda:
-        out = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-        act = torch.empty_like(out)
-        if out.numel():
-            lib().act_unpack(p.data, out, act)
-            count_launch()
-        return out, act
+        count_launch()
+        x, act = lib().unpack(p.data, p.cols, p.dtype == torch.float32, True)
+        return x, act
     x = _values(p)
     return x.to(p.dtype), torch.nn.functional.gelu(x).to(p.dtype)

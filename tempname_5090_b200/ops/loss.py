@@ -107,7 +107,7 @@ class ScoreState:
         self.stats, self.start, self.vocab = stats, start, vocab
 
 
-def _check_scoring(logits, targets):
+def _check_scoring(logits, targets, top_k=0, world=1):
     if logits.dim() != 2 or logits.dtype not in SCORE_DTYPES:
         raise ValueError("logits must be a BF16, FP16 or FP32 matrix [rows, vocabulary]")
     if logits.shape[1] == 0:
@@ -116,9 +116,13 @@ def _check_scoring(logits, targets):
         raise ValueError("logits need contiguous rows")
     if targets.dtype != torch.int64 or targets.shape != logits.shape[:1] or targets.device != logits.device:
         raise ValueError("targets must be int64 [rows] on the logits' device")
+    most = min(MAX_TOP, logits.shape[1])
+    if not 0 <= top_k <= most:
+        raise ValueError(f"top_k must be between 0 and {most}")
+    if logits.shape[1] * world > 2 ** 31 - 1:
+        raise ValueError("the vocabulary must fit 32-bit ids")
 
 
-@torch.no_grad()
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, group=None, rank: int = 0,
                    world: int = 1):
     """Return (TokenScores, ScoreState) of logits [M, V/world] (this rank's shard).
@@ -129,34 +133,34 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
     gradient.  A NaN or +inf makes its row's numbers NaN.  `top_k` is at most 32
     and at most the shard's vocabulary.
     """
-    _check_scoring(logits, targets)
-    M, V = logits.shape
-    if not 0 <= top_k <= min(MAX_TOP, V):
-        raise ValueError(f"top_k must be between 0 and {min(MAX_TOP, V)}")
-    if V * world > 2 ** 31 - 1:
-        raise ValueError("the vocabulary must fit 32-bit ids")
-    start = rank * V
-    dev = logits.device
+    if logits.is_cuda and world == 1:
+        try:
+            logprob, entropy, top, ids, stats = lib().token_logprobs(logits, targets, top_k)
+        except (RuntimeError, TypeError):
+            _check_scoring(logits, targets, top_k)
+            raise
+        count_launch()
+        return TokenScores(logprob, entropy, top, ids), ScoreState(stats, 0, logits.shape[1])
+    _check_scoring(logits, targets, top_k, world)
     if not logits.is_cuda:
         return _token_logprobs_cpu(logits, targets, top_k, group, rank, world)
+    M, V = logits.shape
+    dev = logits.device
     targets = targets.contiguous()
     out = torch.empty(M * (5 + top_k), dtype=torch.float32, device=dev)
     ids = torch.empty((M, top_k), dtype=torch.int64, device=dev)
     if M:
-        if world == 1:
-            lib().score_fwd(logits, targets, 0, V, top_k, out, ids, None)
-            count_launch()
-        else:
-            records = torch.empty((world, M, 4 + 2 * top_k), dtype=torch.float32, device=dev)
-            mine = torch.empty((M, 4 + 2 * top_k), dtype=torch.float32, device=dev)
-            lib().score_fwd(logits, targets, start, V * world, top_k, None, None, mine)
-            dist.all_gather_into_tensor(records, mine, group=group)
-            lib().score_merge(records, targets, V, top_k, out, ids)
-            count_launch(2)
+        records = torch.empty((world, M, 4 + 2 * top_k), dtype=torch.float32, device=dev)
+        mine = torch.empty((M, 4 + 2 * top_k), dtype=torch.float32, device=dev)
+        lib().score_fwd(logits, targets, rank * V, V * world, top_k, None, None, mine)
+        dist.all_gather_into_tensor(records, mine, group=group)
+        lib().score_merge(records, targets, V, top_k, out, ids)
+        count_launch(2)
     scores = TokenScores(out[:M], out[M:2 * M], out[5 * M:].view(M, top_k), ids)
-    return scores, ScoreState(out[2 * M:5 * M].view(3, M), start, V * world)
+    return scores, ScoreState(out[2 * M:5 * M].view(3, M), rank * V, V * world)
 
 
+@torch.no_grad()
 def _token_logprobs_cpu(logits, targets, top_k, group, rank, world):
     """The same numbers in torch, with the same records between ranks."""
     M, V = logits.shape
@@ -197,13 +201,26 @@ def _token_logprobs_cpu(logits, targets, top_k, group, rank, world):
             ScoreState(torch.stack([m, log_s, entropy]), rank * V, V * world))
 
 
-@torch.no_grad()
 def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, state: ScoreState,
                             dlogprob: torch.Tensor, dentropy: torch.Tensor | None = None,
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of the logits [M, V/world] from that of the log probabilities and
     (optional) of the entropies, both FP32 [M].  `out` may be the logits themselves,
     which are dead after the loss; otherwise it must not overlap them."""
+    if logits.is_cuda:
+        try:
+            out = lib().token_logprobs_backward(logits, targets, state.start, state.vocab, state.stats, dlogprob,
+                                                dentropy, out)
+        except (RuntimeError, TypeError):
+            _check_score_gradient(logits, targets, state, dlogprob, dentropy, out)
+            raise
+        count_launch()
+        return out
+    _check_score_gradient(logits, targets, state, dlogprob, dentropy, out)
+    return _score_gradient_cpu(logits, targets, state, dlogprob, dentropy, out)
+
+
+def _check_score_gradient(logits, targets, state, dlogprob, dentropy, out):
     _check_scoring(logits, targets)
     M, V = logits.shape
     for name, t in (("dlogprob", dlogprob), ("dentropy", dentropy)):
@@ -211,17 +228,15 @@ def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, state: 
             raise ValueError(f"{name} must be FP32 [rows] on the logits' device")
     if state.stats.shape != (3, M) or state.stats.device != logits.device:
         raise ValueError("the state belongs to other logits")
-    if out is None:
-        out = torch.empty((M, V), dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
-            or (V > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < V):
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device
+                            or (V > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < V)):
         raise ValueError("out must be like the logits, with contiguous rows of its own")
-    if logits.is_cuda:
-        if M:
-            lib().score_bwd(logits, targets.contiguous(), state.start, state.vocab, state.stats,
-                            dlogprob.contiguous(), None if dentropy is None else dentropy.contiguous(), out)
-            count_launch()
-        return out
+
+
+@torch.no_grad()
+def _score_gradient_cpu(logits, targets, state, dlogprob, dentropy, out):
+    M, V = logits.shape
+    out = torch.empty((M, V), dtype=logits.dtype) if out is None else out
     m, log_s, entropy = state.stats
     empty = m == -torch.inf
     a = torch.where(targets >= 0, dlogprob, torch.zeros(()))

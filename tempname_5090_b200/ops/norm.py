@@ -152,7 +152,6 @@ def _check_kept(name, t, like, shape):
         _check_matrix(name, t, like, shape)
 
 
-@torch.no_grad()
 def block_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps, residual_scale=1.0, out=None):
     """Returns (x_out, h, stats) for the residual stream x and a branch's output y, [rows, H]:
 
@@ -164,23 +163,31 @@ def block_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps
     computed from x_out before its rounding to the storage type.  `stats` (FP32
     [4, rows]: mean and reciprocal deviation of y, then of x_out) is for the gradient.
     """
+    if x.is_cuda:
+        try:
+            x_out, h, stats = lib().block_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias,
+                                                   residual_scale, eps, out)
+        except (RuntimeError, TypeError):
+            _check_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, out)
+            raise
+        count_launch()
+        return x_out, h, stats
+    _check_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, out)
+    return _join_fwd_cpu(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps, residual_scale, out)
+
+
+def _check_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, out):
     _check_first("x", x)
-    rows, H = x.shape
     _check_matrix("x", x, x, x.shape)
     _check_matrix("y", y, x, x.shape)
-    _check_vectors(x, H, post_weight=post_weight, post_bias=post_bias, gate=gate, pre_weight=pre_weight,
+    _check_vectors(x, x.shape[1], post_weight=post_weight, post_bias=post_bias, gate=gate, pre_weight=pre_weight,
                    pre_bias=pre_bias)
     if out is not None:
         _check_matrix("out", out, x, x.shape, own_rows=True)
-    if x.is_cuda:
-        x_out = torch.empty((rows, H), dtype=x.dtype, device=x.device)
-        h = torch.empty_like(x_out) if out is None else out
-        stats = torch.empty((4, rows), dtype=torch.float32, device=x.device)
-        if rows:
-            lib().join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, x_out, h, stats,
-                           float(residual_scale), float(eps))
-            count_launch()
-        return x_out, h, stats
+
+
+@torch.no_grad()
+def _join_fwd_cpu(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps, residual_scale, out):
     yhat, mean_y, rstd_y = _normed(y.float(), eps)
     u = residual_scale * x.float() + gate.float() * (yhat * post_weight.float() + post_bias.float())
     uhat, mean_u, rstd_u = _normed(u, eps)
@@ -205,14 +212,6 @@ def _norm_input_grad(g, hat, rstd):
     return rstd[:, None] * (g - g.mean(1, keepdim=True) - hat * (g * hat).mean(1, keepdim=True))
 
 
-def _join_workspace(workspace, rows, H, branch, device):
-    need = lib().join_bwd_workspace(rows, H, branch)
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.float32, device=device)
-    return workspace
-
-
-@torch.no_grad()
 def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, residual_scale=1.0,
                    pre_bias=None, workspace=None, out=None) -> JoinGrads:
     """Gradients of `block_join_fwd` from that of h and (or None) of x_out.
@@ -223,6 +222,25 @@ def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pr
     is large enough.  Gradients of x_out and h join in FP32; parameter gradients are
     sums over the rows in a fixed order.
     """
+    if dh.is_cuda:
+        try:
+            kept = isinstance(x_out, Packed8)
+            if kept != isinstance(y, Packed8):
+                raise ValueError("x_out and y are kept in the same form")
+            grads = lib().block_join_bwd(dh, dx_out, x_out.data if kept else x_out, y.data if kept else y, stats,
+                                         post_weight, post_bias, gate, pre_weight, pre_bias, out, workspace,
+                                         residual_scale)
+        except (RuntimeError, TypeError):
+            _check_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, pre_bias, out)
+            raise
+        count_launch(2)
+        return JoinGrads(*grads)
+    _check_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, pre_bias, out)
+    return _join_bwd_cpu(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, residual_scale,
+                         pre_bias, out)
+
+
+def _check_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, pre_bias, out):
     _check_first("dh", dh)
     rows, H = dh.shape
     _check_matrix("dh", dh, dh, dh.shape)
@@ -238,20 +256,10 @@ def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pr
         _check_vectors(dh, H, pre_bias=pre_bias)
     if out is not None:
         _check_matrix("out", out, dh, dh.shape, own_rows=True)
-    if dh.is_cuda:
-        dx = torch.empty((rows, H), dtype=dh.dtype, device=dh.device)
-        dy = torch.empty_like(dx) if out is None else out
-        h = None if pre_bias is None else torch.empty_like(dx)
-        grads = torch.empty((5, H), dtype=dh.dtype, device=dh.device)
-        if rows:
-            packed = isinstance(x_out, Packed8)
-            lib().join_bwd(dh, dx_out, x_out.data if packed else x_out, y.data if packed else y, stats[2], stats[3],
-                           stats[0], stats[1], post_weight, post_bias, gate, pre_weight, pre_bias, dx, dy, h, grads,
-                           _join_workspace(workspace, rows, H, True, dh.device), float(residual_scale))
-            count_launch(2)
-        else:
-            grads.zero_()
-        return JoinGrads(dx, dy, grads[2], grads[3], grads[4], grads[0], grads[1], h)
+
+
+@torch.no_grad()
+def _join_bwd_cpu(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, residual_scale, pre_bias, out):
     mean_y, rstd_y, mean_u, rstd_u = stats
     uhat = (_kept_float(x_out) - mean_u[:, None]) * rstd_u[:, None]
     yhat = (_kept_float(y) - mean_y[:, None]) * rstd_y[:, None]
@@ -270,7 +278,6 @@ def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pr
                      (dhf * uhat).sum(0).to(dh.dtype), dhf.sum(0).to(dh.dtype), h)
 
 
-@torch.no_grad()
 def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, workspace=None, out=None):
     """LayerNorm's gradient from its input kept in 8 bits (x: Packed8) and the
     statistics of the forward pass.  Returns (dx, dweight, dbias, y): dx includes
@@ -278,6 +285,21 @@ def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, works
     norm's output again when `bias` is given (the weight gradient of the product that
     follows reads it), else None.
     """
+    if dy.is_cuda:
+        if not isinstance(x, Packed8):
+            raise ValueError("x must be a Packed8")
+        try:
+            dx, dw, db, y = lib().layer_norm_bwd_packed(dy, dres, x.data, mean, rstd, weight, bias, out, workspace)
+        except (RuntimeError, TypeError):
+            _check_packed_norm(dy, x, weight, mean, rstd, dres, bias, out)
+            raise
+        count_launch(2)
+        return dx, dw, db, y
+    _check_packed_norm(dy, x, weight, mean, rstd, dres, bias, out)
+    return _packed_norm_cpu(dy, x, weight, mean, rstd, dres, bias, out)
+
+
+def _check_packed_norm(dy, x, weight, mean, rstd, dres, bias, out):
     _check_first("dy", dy)
     rows, H = dy.shape
     _check_matrix("dy", dy, dy, dy.shape)
@@ -292,17 +314,10 @@ def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, works
         _check_matrix("dres", dres, dy, dy.shape)
     if out is not None:
         _check_matrix("out", out, dy, dy.shape, own_rows=True)
-    if dy.is_cuda:
-        dx = torch.empty((rows, H), dtype=dy.dtype, device=dy.device) if out is None else out
-        y = None if bias is None else torch.empty((rows, H), dtype=dy.dtype, device=dy.device)
-        grads = torch.empty((2, H), dtype=dy.dtype, device=dy.device)
-        if rows:
-            lib().join_bwd(dy, dres, x.data, None, mean, rstd, None, None, None, None, None, weight, bias, dx, None, y,
-                           grads, _join_workspace(workspace, rows, H, False, dy.device), 1.0)
-            count_launch(2)
-        else:
-            grads.zero_()
-        return dx, grads[0], grads[1], y
+
+
+@torch.no_grad()
+def _packed_norm_cpu(dy, x, weight, mean, rstd, dres, bias, out):
     hat = (_values(x) - mean[:, None]) * rstd[:, None]
     g = dy.float()
     dx = _norm_input_grad(g * weight.float(), hat, rstd)

@@ -166,3 +166,11 @@ def gelu(v):
     """v Phi(v) in FP64, by erfc: 1 + erf loses all digits of Phi below about -8."""
     phi = 0.5 * torch.special.erfc(-v * 0.5 ** 0.5)
     return torch.where(v.isinf(), v.clamp(min=0), v * torch.where(v.isinf(), torch.zeros_like(v), phi))
+
+
+def gelu_bound(v, gelu, dtype):
+    """v Phi(v) with Phi in FP32: e^x and erfcx are good to a few steps, 16 half steps in
+    all; and a Phi below 2^-126 (|v| > 13) is itself off by up to half a subnormal step,
+    2^-150, and two more from e^x and the product, all of it times |v|."""
+    size = torch.where(v.isfinite(), v.abs(), torch.zeros_like(v))
+    return rounded(gelu, dtype) + 16 * U * gelu.abs() + size * 3 * 2.0 ** -150

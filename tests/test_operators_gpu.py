@@ -40,7 +40,7 @@ def test_pack_and_unpack(rows, cols, dtype):
     assert torch.equal(v, actpack.unpack(p))
     gelu = ref.gelu(want)
     # e^x and erfcx are good to a few steps of FP32
-    ref.close(act, gelu, ref.rounded(gelu, dtype) + 16 * ref.U * gelu.abs())
+    ref.close(act, gelu, ref.gelu_bound(want, gelu, dtype))
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
@@ -63,8 +63,7 @@ def test_pack_special_values(dtype):
     assert torch.equal(v.nan_to_num(9.0), actpack.unpack(p).nan_to_num(9.0))
     want = ref.kept(x)
     gelu = ref.gelu(want)
-    # below 2^-24 the kernel takes v / 2, off by 0.8 |v| relative
-    ref.close(act, gelu, ref.rounded(gelu, dtype) + 16 * ref.U * gelu.abs())
+    ref.close(act, gelu, ref.gelu_bound(want, gelu, dtype))
 
 
 def test_every_code_under_every_unit():
@@ -83,7 +82,7 @@ def test_every_code_under_every_unit():
     v, act = actpack.unpack_gelu(p)
     ref.close(v, want, torch.zeros((), device="cuda"))
     gelu = ref.gelu(want)
-    ref.close(act, gelu, ref.rounded(gelu, FP32) + 16 * ref.U * gelu.abs())
+    ref.close(act, gelu, ref.gelu_bound(want, gelu, FP32))
 
 
 def test_pack_of_strided_and_unaligned_rows():
