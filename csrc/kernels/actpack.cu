@@ -34,6 +34,25 @@ __device__ __forceinline__ unsigned short encode2(float a, float b, float invers
   return __nv_cvt_float2_to_fp8x2(make_float2(a * inverse, b * inverse), __NV_SATFINITE, __NV_E4M3);
 }
 
+// Eight values to p (on a 16-byte boundary).
+__device__ __forceinline__ void put8(__nv_bfloat16* p, const Two* v) {
+  unsigned w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = both(v[i]);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    w[i] = *reinterpret_cast<const unsigned*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void put8(float* p, const Two* v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = both(v[2 * i]), b = both(v[2 * i + 1]);
+    reinterpret_cast<float4*>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
 // Largest magnitude of eight values, and whether all are finite.
 __device__ __forceinline__ float largest(const Eight<__nv_bfloat16>& e) {
   // Magnitudes of BF16 pairs order like unsigned 16-bit numbers.
@@ -51,9 +70,36 @@ __device__ __forceinline__ float largest(const Eight<float>& e) {
   return m;
 }
 
+// The exponent byte of a group from its values' largest magnitude `amax` over the
+// lanes that share it (LANES of them, N values each); values that the codes cannot
+// hold are replaced on the way.
+template <int LANES, int N>
+__device__ __forceinline__ unsigned settle(float* v, float amax) {
+#pragma unroll
+  for (int d = LANES / 2; d; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(kAllLanes, amax, d));
+  // Ordinary groups end here; the rest (the same for all lanes of a group) takes the long way.
+  const bool odd = !(amax < 240.f * 1.329227996e36f);
+  if (__any_sync(kAllLanes, odd)) {
+    float finite = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) finite = fmaxf(finite, finite_abs(v[i]));
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) finite = fmaxf(finite, __shfl_xor_sync(kAllLanes, finite, d));
+    amax = finite;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // Infinities as NaN have a code of their own; magnitudes past the last code are that code.
+      const float a = fabsf(v[i]);
+      v[i] = a <= 3.402823466e38f ? copysignf(fminf(a, 240.f * 1.329227996e36f), v[i]) : __int_as_float(0x7fffffff);
+    }
+  }
+  return unit_byte(amax);
+}
+__device__ __forceinline__ float inverse_unit(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
+
 // Eight lanes per group; a lane has eight columns of each half, so that every
 // load and store of a group is one contiguous piece.
-template <typename T, bool VEC>
+template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsigned char* data, int cols,
                                                    unsigned groups, unsigned items) {
   const int lane = threadIdx.x & 7;
@@ -63,48 +109,17 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsig
   const int col = int(group) * kPackGroup + lane * 8;
   Eight<T> e[2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
     for (int i = 0; i < int(sizeof(T) / 2); ++i) e[h].raw[i] = make_uint4(0, 0, 0, 0);
-  const T* src = x + int64_t(row) * ld + col;
-  if (VEC) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (live && col + h * 64 < cols) e[h].load_once(src + h * 64);
-  } else if (live) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      T* v = reinterpret_cast<T*>(e[h].raw);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (col + h * 64 + i < cols) v[i] = src[h * 64 + i];
-    }
+    if (live && col + h * 64 < cols) e[h].load_once(x + int64_t(row) * ld + col + h * 64);
   }
-  float amax = max_nan(largest(e[0]), largest(e[1]));
-#pragma unroll
-  for (int d = 4; d; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(kAllLanes, amax, d));
   float v[16];
   e[0].get(v);
   e[1].get(v + 8);
-  // Ordinary groups end here; the rest (the same for a group's eight lanes) takes the long way.
-  const bool odd = !(amax < 240.f * 1.329227996e36f);
-  if (__any_sync(kAllLanes, odd)) {
-    float finite = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) finite = fmaxf(finite, finite_abs(v[i]));
-#pragma unroll
-    for (int d = 4; d; d >>= 1) finite = fmaxf(finite, __shfl_xor_sync(kAllLanes, finite, d));
-    amax = finite;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      // Infinities as NaN have a code of their own; magnitudes past the last code are that code.
-      const float a = fabsf(v[i]);
-      v[i] = a <= 3.402823466e38f ? copysignf(fminf(a, 240.f * 1.329227996e36f), v[i]) : __int_as_float(0x7fffffff);
-    }
-  }
+  const unsigned byte = settle<8, 16>(v, max_nan(largest(e[0]), largest(e[1])));
   if (!live) return;
-  const unsigned byte = unit_byte(amax);
-  const float inverse = __uint_as_float((254u - byte) << 23);
+  const float inverse = inverse_unit(byte);
   unsigned char* dst = data + int64_t(row) * pack_row_bytes(cols);
   const int code_bytes = int(pack_code_bytes(cols));
 #pragma unroll
@@ -124,6 +139,33 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsig
   }
 }
 
+// Odd widths and unaligned rows: a warp per group, single values, contiguous over the warp.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_odd_kernel(const T* x, int64_t ld, unsigned char* data, int cols,
+                                                       unsigned groups, unsigned items) {
+  const int lane = threadIdx.x & 31;
+  const unsigned item = blockIdx.x * 8u + threadIdx.x / 32u;
+  if (item >= items) return;
+  const unsigned row = item / groups, group = item - row * groups;
+  const int col = int(group) * kPackGroup + lane;
+  const T* src = x + int64_t(row) * ld;
+  float v[4], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = col + i * 32 < cols ? to_float(src[col + i * 32]) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = max_nan(amax, fabsf(v[i]));
+  const unsigned byte = settle<32, 4>(v, amax);
+  const float inverse = inverse_unit(byte);
+  unsigned char* dst = data + int64_t(row) * pack_row_bytes(cols);
+  const int code_bytes = int(pack_code_bytes(cols));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i * 32 < code_bytes) dst[col + i * 32] = static_cast<unsigned char>(encode2(v[i], 0.f, inverse) & 0xffu);
+  unsigned char* units = dst + code_bytes;
+  if (lane == 0) units[group] = static_cast<unsigned char>(byte);
+  if (group == groups - 1 && groups + lane < (groups + 15u) / 16u * 16u) units[groups + lane] = 0;
+}
+
 // GeLU(v) = v * Phi(v) of a kept value.  Kept values have three mantissa bits, so
 // binade and mantissa (eight entries a binade) and the sign name each of them: a
 // table of Phi over the magnitudes 2^-24 .. 2^8 replaces the error function, which
@@ -131,9 +173,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsig
 // mantissa in bits 7 to 14 and the sign above; the group's unit moves the binade,
 // that is, the place in the table: entry = bits 7..15 + 8 (e + 9).  Zeros have no
 // binade and hit any entry (or the padding below), times zero.
-// Table: [pad | positive 256 | negative 256 | end], the end for the NaN codes.
+// Table: [pad | positive 256 | negative 256 | end], the end for the NaN codes.  Eight
+// copies, one for every eighth lane, side by side: an entry's copies lie in eight
+// banks, so only four lanes can meet in a bank.
 constexpr int kTablePad = 48, kTableHalf = 256, kTableEnd = 64, kTableLow = 127 - 24;
-constexpr int kTableSize = kTablePad + 2 * kTableHalf + kTableEnd;
+constexpr int kTableSize = kTablePad + 2 * kTableHalf + kTableEnd, kCopies = 8;
 __device__ __forceinline__ void fill_phi_table(float* table) {
   for (int i = threadIdx.x; i < kTableSize; i += blockDim.x) {
     const int k = i - kTablePad;
@@ -142,7 +186,10 @@ __device__ __forceinline__ void fill_phi_table(float* table) {
     // FP32 (v has four significant bits), where erfc of a rounded argument would be
     // off by v^2 roundings.
     const float z = 0.70710678118654752440f * v;
-    table[i] = k < 0 ? 0.5f : k < kTableHalf ? 0.5f * erfcf(-z) : 0.5f * expf(-0.5f * v * v) * erfcxf(z);
+    const float phi = k < 0 ? 0.5f : k < kTableHalf ? 0.5f * erfcf(-z) : 0.5f * expf(-0.5f * v * v) * erfcxf(z);
+    const float4 four = make_float4(phi, phi, phi, phi);
+    reinterpret_cast<float4*>(table)[2 * i] = four;
+    reinterpret_cast<float4*>(table)[2 * i + 1] = four;
   }
 }
 // Any kept value, from its FP32 bits.
@@ -151,69 +198,113 @@ __device__ __forceinline__ float kept_gelu(float v, const float* table) {
   const int k = int((bits >> 20) & 0x7ffu) - kTableLow * 8;
   if (k < 0) return 0.5f * v;                                     // Phi(v) = 1/2 within 2^-24
   if (k >= kTableHalf) return v > 0.f ? v : (v == v ? -0.f : v);  // Phi(-256) = 0
-  return v * table[kTablePad + k + int(bits >> 31) * kTableHalf];
+  return v * table[(kTablePad + k + int(bits >> 31) * kTableHalf) * kCopies];
 }
 
-// Sixteen columns per thread (one 16-byte load of codes).
-template <typename T, bool GELU, bool VEC>
+// Sixteen columns per thread and step (one 16-byte load of codes), two steps at once.
+template <typename T, bool GELU>
 __global__ void __launch_bounds__(256) unpack_kernel(const unsigned char* data, T* out, T* act, int cols,
                                                      unsigned segments, unsigned items) {
-  __shared__ float table[GELU ? kTableSize : 1];
+  __shared__ __align__(16) float table[GELU ? kTableSize * kCopies : 4];
+  const int64_t row_bytes = pack_row_bytes(cols);
+  const int code_bytes = int(pack_code_bytes(cols));
+  const unsigned stride = gridDim.x * 256u;
+  constexpr int kSteps = 2;
+  bool ready = !GELU;
+  for (unsigned first = blockIdx.x * 256u + threadIdx.x; first < items || !ready; first += kSteps * stride) {
+    uint4 codes[kSteps];
+    unsigned byte[kSteps], row[kSteps];
+    int col[kSteps];
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const unsigned item = first + k * stride;
+      codes[k] = make_uint4(0, 0, 0, 0);
+      byte[k] = 1;
+      row[k] = item / segments;
+      col[k] = int(item - row[k] * segments) * 16;
+      if (item < items) {
+        const unsigned char* src = data + int64_t(row[k]) * row_bytes;
+        codes[k] = __ldcs(reinterpret_cast<const uint4*>(src + col[k]));
+        byte[k] = src[code_bytes + col[k] / kPackGroup];
+      }
+    }
+    if (!ready) {  // the table is filled while the first codes are on their way
+      fill_phi_table(table);
+      __syncthreads();
+      ready = true;
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      if (first + k * stride >= items) break;
+      const float unit = pack_unit(byte[k]);
+      const unsigned words[4] = {codes[k].x, codes[k].y, codes[k].z, codes[k].w};
+      // e in [-15, -1]: every code's binade lies in the table's window.
+      const bool window = byte[k] - 112u <= 14u;
+      const char* place = reinterpret_cast<const char*>(
+          table + (kTablePad + 8 * (int(byte[k]) - 127 + 9)) * kCopies + (threadIdx.x & (kCopies - 1)));
+      Two v[8], a[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned short code2 = i & 1 ? words[i / 2] >> 16 : words[i / 2] & 0xffffu;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(code2), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        v[i] = two_mul(two(f.x, f.y), two(unit, unit));
+        if (GELU && window) {
+          // Bits 7 .. 15 as an entry of 32 bytes: bits 5 .. 13 of the offset.
+          const unsigned w = unsigned(h.y) << 16 | h.x;
+          const float lo = *reinterpret_cast<const float*>(place + ((w >> 2) & 0x3fe0u));
+          const float hi = *reinterpret_cast<const float*>(place + ((w >> 18) & 0x3fe0u));
+          a[i] = two_mul(v[i], two(lo, hi));
+        }
+      }
+      if (GELU && !window) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = both(v[i]);
+          a[i] = two(kept_gelu(f.x, table), kept_gelu(f.y, table));
+        }
+      }
+      T* o = out + int64_t(row[k]) * cols + col[k];
+      T* g = act + int64_t(row[k]) * cols + col[k];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (col[k] + h * 8 >= cols) break;
+        put8(o + h * 8, v + h * 4);
+        if (GELU) put8(g + h * 8, a + h * 4);
+      }
+    }
+  }
+}
+
+// Odd widths and unaligned outputs: a warp has 512 columns, 32 at a time, so that
+// loads and stores of single values are still contiguous over the warp.
+template <typename T, bool GELU>
+__global__ void __launch_bounds__(256) unpack_odd_kernel(const unsigned char* data, T* out, T* act, int cols,
+                                                         unsigned segments, unsigned items) {
+  __shared__ __align__(16) float table[GELU ? kTableSize * kCopies : 4];
   if (GELU) {
     fill_phi_table(table);
     __syncthreads();
   }
   const int64_t row_bytes = pack_row_bytes(cols);
-  const int code_bytes = int(pack_code_bytes(cols));
-  for (unsigned item = blockIdx.x * 256u + threadIdx.x; item < items; item += gridDim.x * 256u) {
+  const int code_bytes = int(pack_code_bytes(cols)), lane = threadIdx.x & 31;
+  for (unsigned item = blockIdx.x * 8u + threadIdx.x / 32u; item < items; item += gridDim.x * 8u) {
     const unsigned row = item / segments;
-    const int col = int(item - row * segments) * 16;
+    const int col = int(item - row * segments) * 512 + lane;
     const unsigned char* src = data + int64_t(row) * row_bytes;
-    const uint4 codes = *reinterpret_cast<const uint4*>(src + col);
-    const unsigned byte = src[code_bytes + col / kPackGroup];
-    const float unit = pack_unit(byte);
-    const unsigned words[4] = {codes.x, codes.y, codes.z, codes.w};
-    // e in [-15, -1]: every code's binade lies in the table's window.
-    const bool window = byte - 112u <= 14u;
-    const float* place = table + kTablePad + 8 * (int(byte) - 127 + 9);
-    float v[16], a[16];
+    unsigned char code[16], byte[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned short code2 = i & 1 ? words[i / 2] >> 16 : words[i / 2] & 0xffffu;
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(code2), __NV_E4M3);
-      const float2 f = __half22float2(__half2(h));
-      v[2 * i] = f.x * unit;
-      v[2 * i + 1] = f.y * unit;
-      if (GELU && window) {
-        a[2 * i] = v[2 * i] * place[(h.x >> 7) & 0x1ff];
-        a[2 * i + 1] = v[2 * i + 1] * place[h.y >> 7];
-      }
+    for (int i = 0; i < 16; ++i) {
+      if ((i & 3) == 0) byte[i / 4] = col + i * 32 < cols ? src[code_bytes + (col + i * 32) / kPackGroup] : 1;
+      code[i] = col + i * 32 < cols ? src[col + i * 32] : 0;
     }
-    if (GELU && !window) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) a[i] = kept_gelu(v[i], table);
-    }
-    T* o = out + int64_t(row) * cols + col;
-    T* g = act + int64_t(row) * cols + col;
-    if (VEC) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (col + h * 8 >= cols) break;
-        Eight<T> e;
-        e.set(v + h * 8);
-        e.store(o + h * 8);
-        if (GELU) {
-          e.set(a + h * 8);
-          e.store(g + h * 8);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (col + i >= cols) break;
-        o[i] = from_float<T>(v[i]);
-        if (GELU) g[i] = from_float<T>(a[i]);
-      }
+    for (int i = 0; i < 16; ++i) {
+      if (col + i * 32 >= cols) break;
+      const float v = decode1(code[i], pack_unit(byte[i / 4]));
+      const int64_t at = int64_t(row) * cols + col + i * 32;
+      out[at] = from_float<T>(v);
+      if (GELU) act[at] = from_float<T>(kept_gelu(v, table));
     }
   }
 }
@@ -224,27 +315,26 @@ template <typename T>
 int pack_typed(const void* x, int64_t ld, void* data, int64_t rows, int64_t cols, cudaStream_t s) {
   const int64_t groups = pack_groups(cols), items = rows * groups;
   const bool vec = cols % 8 == 0 && ld * int64_t(sizeof(T)) % 16 == 0 && aligned16(x);
-  const unsigned grid = unsigned((items + 31) / 32);
-  auto launch = [&](auto kernel) {
-    kernel<<<grid, 256, 0, s>>>(static_cast<const T*>(x), ld, static_cast<unsigned char*>(data), int(cols),
-                                unsigned(groups), unsigned(items));
+  auto launch = [&](auto kernel, int64_t per_cta) {
+    kernel<<<unsigned((items + per_cta - 1) / per_cta), 256, 0, s>>>(
+        static_cast<const T*>(x), ld, static_cast<unsigned char*>(data), int(cols), unsigned(groups), unsigned(items));
   };
-  vec ? launch(pack_kernel<T, true>) : launch(pack_kernel<T, false>);
+  vec ? launch(pack_kernel<T>, 32) : launch(pack_odd_kernel<T>, 8);
   return int(cudaGetLastError());
 }
 
 template <typename T, bool GELU>
 int unpack_typed(const void* data, void* out, void* act, int64_t rows, int64_t cols, cudaStream_t s) {
-  const int64_t segments = (cols + 15) / 16, items = rows * segments;
   const bool vec = cols % 8 == 0 && aligned16(out) && (!GELU || aligned16(act));
+  const int64_t segments = vec ? (cols + 15) / 16 : (cols + 511) / 512, items = rows * segments;
   if (items > 0x7fffffff) return -1;
-  int64_t grid = (items + 255) / 256;
-  if (GELU && grid > 148 * 8) grid = 148 * 8;  // one table for many rows
+  const int64_t ctas = vec ? (items + 511) / 512 : (items + 7) / 8;
+  const unsigned grid = unsigned(ctas < 148 * 5 ? ctas : 148 * 5);  // five CTAs an SM: one table for many rows
   auto launch = [&](auto kernel) {
-    kernel<<<unsigned(grid), 256, 0, s>>>(static_cast<const unsigned char*>(data), static_cast<T*>(out),
-                                          static_cast<T*>(act), int(cols), unsigned(segments), unsigned(items));
+    kernel<<<grid, 256, 0, s>>>(static_cast<const unsigned char*>(data), static_cast<T*>(out), static_cast<T*>(act),
+                                int(cols), unsigned(segments), unsigned(items));
   };
-  vec ? launch(unpack_kernel<T, GELU, true>) : launch(unpack_kernel<T, GELU, false>);
+  vec ? launch(unpack_kernel<T, GELU>) : launch(unpack_odd_kernel<T, GELU>);
   return int(cudaGetLastError());
 }
 }  // namespace

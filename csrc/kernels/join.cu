@@ -14,9 +14,22 @@
 //   Q = sum dt: dg = pw P + pb Q, dpw = g P, dpb = g Q (g, pw, pb are constant
 //   down a column, so two column sums serve three gradients)
 //
-// <.> is the mean over the row.  All arithmetic is FP32; column sums add a fixed
-// set of rows per CTA in order and then the CTAs in order, without atomics.
+// <.> is the mean over the row.  All arithmetic is FP32, two elements an
+// instruction (f32x2); column sums add a fixed set of rows per CTA in order and then
+// the CTAs in order, without atomics.
+//
+// Both directions are persistent: a CTA takes the rows row, row + grid, .. and has
+// the next two on their way into shared memory (cp.async) while it works on one, so
+// loads are in flight all the time and no register holds them.
+//   Vector form (width a multiple of 8, rows on 16-byte boundaries): a thread has
+// eight consecutive columns at a time and copies what it will read itself, so it
+// waits for its own copies alone.
+//   Otherwise (odd widths, views) the CTA copies the 16-byte pieces that cover the
+// row, and threads read single values at the row's offset, columns a CTA's width
+// apart: one barrier more a row.
+#include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kernels_api.h"
 #include "rowvec.cuh"
@@ -24,406 +37,523 @@
 namespace tn5b {
 namespace kernels {
 namespace {
-constexpr int kMaxWarps = 16;
-constexpr int kMaxRing = 200 * 1024;  // of an SM's 227 KB; two rings of half that share an SM
+constexpr int kMaxRing = 200 * 1024;  // of an SM's 227 KB, for all CTAs on it
+constexpr int kStages = 3;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Sums of N values over the CTA, the same bits in every thread.
-template <int N>
-__device__ __forceinline__ void block_sums(float (&v)[N], float (*sh)[kMaxWarps]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+// ------------------------------------------------------- sums over the CTA
+// The same bits in every thread.  `sh` is read by every thread after a barrier; it
+// may be written again after another one.
+template <int NT>
+__device__ __forceinline__ float cta_sum(float v, float* sh) {
+  v = warp_sum(v);
+  if constexpr (NT > 32) {
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if (warps == 1) return;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) sh[i][warp] = v[i];
+    for (int w = 0; w < NT / 128; ++w) {
+      const float4 q = reinterpret_cast<const float4*>(sh)[w];
+      v += (q.x + q.y) + (q.z + q.w);
+    }
   }
-  __syncthreads();
+  return v;
+}
+// Two sums at once: half the warp finishes each.
+template <int NT>
+__device__ __forceinline__ float2 cta_sum2(float a, float b, float2* sh) {
+  const bool high = threadIdx.x & 16;
+  float v = (high ? b : a) + __shfl_xor_sync(kAllLanes, high ? a : b, 16);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float s = 0.f;
-    for (int w = 0; w < warps; ++w) s += sh[i][w];
-    v[i] = s;
+  for (int d = 8; d; d >>= 1) v += __shfl_xor_sync(kAllLanes, v, d);
+  if constexpr (NT == 32) {
+    return make_float2(__shfl_sync(kAllLanes, v, 0), __shfl_sync(kAllLanes, v, 16));
+  } else {
+    if ((threadIdx.x & 15) == 0) reinterpret_cast<float*>(sh)[threadIdx.x >> 4] = v;
+    __syncthreads();
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      const float4 q = reinterpret_cast<const float4*>(sh)[w];
+      s.x += q.x + q.z;
+      s.y += q.y + q.w;
+    }
+    return s;
   }
 }
-
-// Columns of a thread: NV groups of eight.  Vector form: eight consecutive
-// columns; otherwise (odd widths, unaligned rows) columns a CTA's width apart.
-template <int NV, bool VEC>
-struct Columns {
-  int cols;
-  __device__ __forceinline__ int at(int i) const {
-    return VEC ? ((i / 8) * int(blockDim.x) + int(threadIdx.x)) * 8 + (i & 7)
-               : i * int(blockDim.x) + int(threadIdx.x);
-  }
-  __device__ __forceinline__ bool has(int i) const { return at(VEC ? i & ~7 : i) < cols; }
-  template <typename T>
-  __device__ __forceinline__ void load8(const T* row, int g, float* v) const {
-    if (VEC) {
-      Eight<T> e;
-      if (has(g * 8)) {
-        e.load(row + at(g * 8));
-        e.get(v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = has(g * 8 + i) ? to_float(row[at(g * 8 + i)]) : 0.f;
-    }
-  }
-  template <typename T>
-  __device__ __forceinline__ void store8(T* row, int g, const float* v) const {
-    if (VEC) {
-      if (!has(g * 8)) return;
-      Eight<T> e;
-      e.set(v);
-      e.store(row + at(g * 8));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (has(g * 8 + i)) row[at(g * 8 + i)] = from_float<T>(v[i]);
-    }
-  }
-};
-
-// A thread's columns of one row as they were loaded (zeros past the width).
-template <typename T, int NV, bool VEC>
-struct Row {
-  Eight<T> e[NV];
-  __device__ __forceinline__ void load(const Columns<NV, VEC>& c, const T* row, bool once) {
-#pragma unroll
-    for (int g = 0; g < NV; ++g) {
-#pragma unroll
-      for (int i = 0; i < int(sizeof(T) / 2); ++i) e[g].raw[i] = make_uint4(0, 0, 0, 0);
-      if (VEC) {
-        if (c.has(g * 8)) once ? e[g].load_once(row + c.at(g * 8)) : e[g].load(row + c.at(g * 8));
-      } else {
-        T* v = reinterpret_cast<T*>(e[g].raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c.has(g * 8 + i)) v[i] = row[c.at(g * 8 + i)];
-      }
-    }
-  }
-  __device__ __forceinline__ void get(int g, float* v) const { e[g].get(v); }
-};
-struct JoinFwd {
-  const void *x, *y, *pw, *pb, *gate, *w, *b;
-  void *u, *h;
-  float* stats;  // [4][rows]: mean_y, rstd_y, mean_u, rstd_u
-  int64_t ld_x, ld_y, ld_h;
-  int rows, cols;
-  float alpha, eps;
-};
-
-// Mean and reciprocal deviation of the row, from two passes over registers.
-template <int NV, bool VEC>
-__device__ __forceinline__ void row_stats(const Columns<NV, VEC>& c, const float (&v)[NV * 8], float eps, float& mean,
-                                          float& rstd, float (*sh)[kMaxWarps]) {
-  float s[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NV * 8; ++i) s[0] += v[i];
-  block_sums(s, sh);
-  mean = s[0] / c.cols;
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV * 8; ++i) {
-    const float d = v[i] - mean;
-    if (c.has(i)) s[0] = fmaf(d, d, s[0]);
-  }
-  block_sums(s, sh + 1);
-  rstd = rsqrtf(s[0] / c.cols + eps);
+__device__ __forceinline__ float total(Two v) {
+  const float2 f = both(v);
+  return f.x + f.y;
 }
 
-// One CTA a row.  Every thread keeps its columns of y and x as loaded, later of u in
-// FP32.  The vectors over the columns (norm weights, biases, gate) come from L1 for
-// every row but the CTA's SM's first; the rows themselves bypass it.
-template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(256) join_fwd_kernel(JoinFwd p) {
-  __shared__ float sh[4][kMaxWarps];
-  const Columns<NV, VEC> c{p.cols};
-  const int64_t row = blockIdx.x;
-  float y[NV * 8];
-  Row<T, NV, VEC> x;
-  {
-    Row<T, NV, VEC> r;
-    r.load(c, static_cast<const T*>(p.y) + row * p.ld_y, true);
-    x.load(c, static_cast<const T*>(p.x) + row * p.ld_x, true);
+// -------------------------------------------------- eight values as four pairs
+template <typename T> struct Conv;
+template <> struct Conv<__nv_bfloat16> {
+  static __device__ __forceinline__ void get(const uint4* r, Two* v) {
+    const unsigned w[4] = {r->x, r->y, r->z, r->w};
 #pragma unroll
-    for (int g = 0; g < NV; ++g) r.get(g, y + g * 8);
+    for (int i = 0; i < 4; ++i) v[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  float mean, rstd;
-  row_stats(c, y, p.eps, mean, rstd, sh);
-  if (threadIdx.x == 0) {
-    p.stats[row] = mean;
-    p.stats[p.rows + row] = rstd;
-  }
+  static __device__ __forceinline__ void put(const Two* v, uint4* r) {
+    unsigned w[4];
 #pragma unroll
-  for (int g = 0; g < NV; ++g) {
-    float pw[8], pb[8], gate[8], v[8];
-    c.load8(static_cast<const T*>(p.pw), g, pw);
-    c.load8(static_cast<const T*>(p.pb), g, pb);
-    c.load8(static_cast<const T*>(p.gate), g, gate);
-    x.get(g, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float n = fmaf((y[g * 8 + i] - mean) * rstd, pw[i], pb[i]);
-      y[g * 8 + i] = fmaf(gate[i], n, p.alpha * v[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = both(v[i]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+      w[i] = *reinterpret_cast<const unsigned*>(&h);
     }
-    c.store8(static_cast<T*>(p.u) + row * p.cols, g, y + g * 8);
+    *r = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  row_stats(c, y, p.eps, mean, rstd, sh + 2);
-  if (threadIdx.x == 0) {
-    p.stats[2 * int64_t(p.rows) + row] = mean;
-    p.stats[3 * int64_t(p.rows) + row] = rstd;
-  }
+};
+template <> struct Conv<float> {
+  static __device__ __forceinline__ void get(const uint4* r, Two* v) {
 #pragma unroll
-  for (int g = 0; g < NV; ++g) {
-    float w[8], b[8];
-    c.load8(static_cast<const T*>(p.w), g, w);
-    c.load8(static_cast<const T*>(p.b), g, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = fmaf((y[g * 8 + i] - mean) * rstd, w[i], b[i]);
-    c.store8(static_cast<T*>(p.h) + row * p.ld_h, g, b);
+    for (int i = 0; i < 2; ++i) {
+      v[2 * i] = two(__uint_as_float(r[i].x), __uint_as_float(r[i].y));
+      v[2 * i + 1] = two(__uint_as_float(r[i].z), __uint_as_float(r[i].w));
+    }
   }
-}
-
-struct JoinBwd {
-  const void *dh, *du, *u, *y;  // du may be null; u and y rows are packed in the 8-bit form
-  const void *pw, *gate, *w, *b;  // b: only for h
-  const float *mean_y, *rstd_y, *mean_u, *rstd_u;
-  void *dx, *dy, *h;              // h (optional): the norm's output again
-  float* sums;                    // [grid][2 or 4][cols]
-  int64_t ld_dh, ld_du, ld_u, ld_y, ld_dy, ld_dx;
-  int rows, cols;
-  float alpha;
+  static __device__ __forceinline__ void put(const Two* v, uint4* r) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 a = both(v[2 * i]), b = both(v[2 * i + 1]);
+      r[i] = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+    }
+  }
 };
 
-__device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes) {
+// ------------------------------------------------------------- asynchronous copies
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
   const unsigned d = unsigned(__cvta_generic_to_shared(dst));
-  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-  else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void copies_begin() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// The rows that a CTA works on next, in shared memory.  A thread copies the columns
-// that it will read itself, so waiting for its own copies is all that is needed:
-// no barrier, and no register holds a row in flight.
-template <typename T, int NV, bool BRANCH, bool PACKED, int STAGES>
-struct Ring {
-  static constexpr int kWhole = 8 * int(sizeof(T));          // eight values
-  static constexpr int kKept = PACKED ? 8 : kWhole;          // eight values of u or y
-  static constexpr int kGroup = 2 * kWhole + (BRANCH ? 2 : 1) * (kKept + (PACKED ? 4 : 0));
-  static constexpr int bytes(int threads) { return threads * NV * kGroup * STAGES; }
-  char* base;
-  // Arrays of [NV][threads] pieces of at most 16 bytes, one after another in a stage.
-  __device__ __forceinline__ char* piece(int stage, int offset, int g, int size) const {
-    return base + (int64_t(stage) * kGroup + offset) * NV * blockDim.x + (g * int(blockDim.x) + int(threadIdx.x)) * size;
+// A [rows][cols] matrix with a row stride in elements (bytes if packed).
+struct Matrix {
+  const void* data;
+  int64_t ld;
+};
+
+// Columns of thread `tid`, by groups of eight (VEC) or a CTA's width apart, and a
+// matrix's row: copied to `region` of shared memory, read from there, or written.
+template <typename T, int NT, int NV, bool VEC>
+struct Tile {
+  static constexpr int kPieces = int(sizeof(T)) / 2;
+  static __host__ __device__ constexpr int bytes(int cols) {
+    return VEC ? NT * NV * 8 * int(sizeof(T)) : ((cols * int(sizeof(T)) + 15) / 16 + 1) * 16;
   }
-  static constexpr int kDh = 0, kDu = kWhole, kU = 2 * kWhole, kY = kU + kKept, kUnitU = kU + (BRANCH ? 2 : 1) * kKept,
-                       kUnitY = kUnitU + 4;
-  __device__ __forceinline__ void whole(int stage, int offset, int g, const T* src) const {
-#pragma unroll
-    for (int i = 0; i < kWhole / 16; ++i)
-      copy_async(piece(stage, offset + i * 16, g, 16), reinterpret_cast<const char*>(src) + i * 16, 16);
+  static __device__ __forceinline__ int column(int g, int i = 0) {
+    return VEC ? (g * NT + int(threadIdx.x)) * 8 + i : (g * 8 + i) * NT + int(threadIdx.x);
   }
-  __device__ __forceinline__ void kept(int stage, int offset, int unit, int g, const void* row, int col, int cols) const {
-    if constexpr (PACKED) {
-      const unsigned char* r = static_cast<const unsigned char*>(row);
-      copy_async(piece(stage, offset, g, 8), r + col, 8);
-      copy_async(piece(stage, unit, g, 4), r + pack_code_bytes(cols) + (col / kPackGroup & ~3), 4);
-    } else {
-      whole(stage, offset, g, static_cast<const T*>(row) + col);
-    }
+  static __device__ __forceinline__ const T* row_of(const Matrix& m, int64_t row) {
+    return static_cast<const T*>(m.data) + row * m.ld;
   }
-  __device__ __forceinline__ void fetch(const JoinBwd& p, const Columns<NV, true>& c, int64_t row, int stage) const {
-    if (row < p.rows) {
+  static __device__ __forceinline__ void fetch(char* region, const Matrix& m, int64_t row, int rows, int cols) {
+    const T* r = row_of(m, row);
+    if constexpr (VEC) {
 #pragma unroll
       for (int g = 0; g < NV; ++g) {
-        if (!c.has(g * 8)) continue;
-        const int col = c.at(g * 8);
-        whole(stage, kDh, g, static_cast<const T*>(p.dh) + row * p.ld_dh + col);
-        kept(stage, kU, kUnitU, g, static_cast<const char*>(p.u) + row * p.ld_u * (PACKED ? 1 : sizeof(T)), col, p.cols);
-        if (p.du) whole(stage, kDu, g, static_cast<const T*>(p.du) + row * p.ld_du + col);
-        if (BRANCH)
-          kept(stage, kY, kUnitY, g, static_cast<const char*>(p.y) + row * p.ld_y * (PACKED ? 1 : sizeof(T)), col, p.cols);
+        if (column(g) >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          copy_async<16>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16,
+                         reinterpret_cast<const uint4*>(r + column(g)) + i);
+      }
+    } else {
+      // Pieces that reach past the matrix's first or last value are copied value by value.
+      const uintptr_t at = reinterpret_cast<uintptr_t>(r) & ~uintptr_t(15);
+      const int pieces = int((reinterpret_cast<uintptr_t>(r + cols) - at + 15) / 16);
+      const uintptr_t begin = reinterpret_cast<uintptr_t>(m.data),
+                      end = begin + ((rows - 1) * m.ld + cols) * int64_t(sizeof(T));
+      for (int i = threadIdx.x; i < pieces; i += NT) {
+        const uintptr_t src = at + uintptr_t(i) * 16;
+        if (src >= begin && src + 16 <= end) {
+          copy_async<16>(region + i * 16, reinterpret_cast<const void*>(src));
+        } else {
+          for (int b = 0; b < 16; b += int(sizeof(T)))
+            if (src + b >= begin && src + b < end)
+              *reinterpret_cast<T*>(region + i * 16 + b) = *reinterpret_cast<const T*>(src + b);
+        }
       }
     }
-    copies_begin();
   }
-  __device__ __forceinline__ void get_whole(int stage, int offset, int g, float* v) const {
-    Eight<T> e;
+  // Group g of the row in `region`; zeros past the width.
+  static __device__ __forceinline__ void get(const char* region, const Matrix& m, int64_t row, int cols, int g, Two* v) {
+    if constexpr (VEC) {
+      uint4 raw[kPieces];
 #pragma unroll
-    for (int i = 0; i < kWhole / 16; ++i) e.raw[i] = *reinterpret_cast<const uint4*>(piece(stage, offset + i * 16, g, 16));
-    e.get(v);
-  }
-  __device__ __forceinline__ void get_kept(int stage, int offset, int unit, int g, int col, float* v) const {
-    if constexpr (PACKED) {
-      const unsigned four = *reinterpret_cast<const unsigned*>(piece(stage, unit, g, 4));
-      const unsigned byte = four >> (8 * (col / kPackGroup & 3)) & 0xffu;
-      decode8(*reinterpret_cast<const uint2*>(piece(stage, offset, g, 8)), pack_unit(byte), v);
+      for (int i = 0; i < kPieces; ++i)
+        raw[i] = column(g) < cols ? *reinterpret_cast<const uint4*>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16)
+                                  : make_uint4(0, 0, 0, 0);
+      Conv<T>::get(raw, v);
     } else {
-      get_whole(stage, offset, g, v);
+      const T* r = reinterpret_cast<const T*>(region + (reinterpret_cast<uintptr_t>(row_of(m, row)) & 15));
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = column(g, i) < cols ? to_float(r[column(g, i)]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  // Group g of a vector over the columns, from global memory (L1 after the first row).
+  static __device__ __forceinline__ void vector(const void* base, int cols, int g, Two* v) {
+    const T* p = static_cast<const T*>(base);
+    if constexpr (VEC) {
+      uint4 raw[kPieces];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        raw[i] = column(g) < cols ? __ldg(reinterpret_cast<const uint4*>(p + column(g)) + i) : make_uint4(0, 0, 0, 0);
+      Conv<T>::get(raw, v);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = column(g, i) < cols ? to_float(p[column(g, i)]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  static __device__ __forceinline__ void store(void* base, int64_t ld, int64_t row, int cols, int g, const Two* v) {
+    T* p = static_cast<T*>(base) + row * ld;
+    if constexpr (VEC) {
+      if (column(g) >= cols) return;
+      uint4 raw[kPieces];
+      Conv<T>::put(v, raw);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p + column(g))[i] = raw[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = both(v[i]);
+        if (column(g, 2 * i) < cols) p[column(g, 2 * i)] = from_float<T>(f.x);
+        if (column(g, 2 * i + 1) < cols) p[column(g, 2 * i + 1)] = from_float<T>(f.y);
+      }
     }
   }
 };
 
-// One CTA per set of rows (row, row + grid, ..), its column sums in registers.  A row
-// takes two CTA-wide reductions, the second one of values that the first decides.
-// Vector form: the next STAGES - 1 rows are on their way into shared memory meanwhile.
-template <typename T, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
-__global__ void __launch_bounds__(NV == 1 ? 128 : 512, NV == 1 ? 4 : 1) join_bwd_kernel(JoinBwd p) {
-  constexpr int N = NV * 8;
-  extern __shared__ __align__(16) char dynamic[];
-  __shared__ float sh[4][kMaxWarps];
-  const Columns<NV, VEC> c{p.cols};
-  using R = Ring<T, NV, BRANCH, PACKED, STAGES>;
-  const R ring{dynamic};
-  float dw[N], db[N], P[BRANCH ? N : 1], Q[BRANCH ? N : 1];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    dw[i] = db[i] = 0.f;
-    if (BRANCH) P[i] = Q[i] = 0.f;
+// The same of packed rows.  Vector form: eight codes and the four exponent bytes with
+// the group's own among them; otherwise the whole row (it starts on a boundary).
+template <int NT, int NV, bool VEC>
+struct PackedTile {
+  using C = Tile<float, NT, NV, VEC>;
+  static __host__ __device__ constexpr int bytes(int cols) {
+    return VEC ? NT * NV * 12 : int(pack_row_bytes(cols));
   }
-  const int64_t first = blockIdx.x, step = gridDim.x;
-  if constexpr (VEC) {
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) ring.fetch(p, c, first + s * step, s);
-  }
-  int stage = 0;
-  for (int64_t row = first; row < p.rows; row += step) {
-    const float mean_u = p.mean_u[row], rstd_u = p.rstd_u[row];
-    float mean_y = 0.f, rstd_y = 0.f;
-    if (BRANCH) {
-      mean_y = p.mean_y[row];
-      rstd_y = p.rstd_y[row];
-    }
+  static __device__ __forceinline__ void fetch(char* region, const Matrix& m, int64_t row, int, int cols) {
+    const char* r = static_cast<const char*>(m.data) + row * m.ld;
     if constexpr (VEC) {
-      ring.fetch(p, c, row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
-      copies_wait<STAGES - 1>();
-    }
-    auto get_t = [&](const void* base, int64_t ld, int offset, int g, float* v) {
-      if constexpr (VEC) {
-        if (c.has(g * 8)) {
-          ring.get_whole(stage, offset, g, v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-      } else {
-        c.load8(static_cast<const T*>(base) + row * ld, g, v);
-      }
-    };
-    auto get_kept = [&](const void* base, int64_t ld, int offset, int unit, int g, float* v) {
-      if constexpr (VEC) {
-        if (c.has(g * 8)) {
-          ring.get_kept(stage, offset, unit, g, c.at(g * 8), v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-      } else if constexpr (PACKED) {
-        const unsigned char* r = static_cast<const unsigned char*>(base) + row * ld;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = c.at(g * 8 + i);
-          v[i] = c.has(g * 8 + i) ? decode1(r[col], pack_unit(r[pack_code_bytes(p.cols) + col / kPackGroup])) : 0.f;
-        }
-      } else {
-        c.load8(static_cast<const T*>(base) + row * ld, g, v);
-      }
-    };
-    float hat[N], a[N];
-    float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      float d[8], w[8];
-      get_t(p.dh, p.ld_dh, R::kDh, g, d);
-      get_kept(p.u, p.ld_u, R::kU, R::kUnitU, g, hat + g * 8);
-      c.load8(static_cast<const T*>(p.w), g, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = g * 8 + i;
-        hat[k] = (hat[k] - mean_u) * rstd_u;
-        dw[k] = fmaf(d[i], hat[k], dw[k]);
-        db[k] += d[i];
-        a[k] = d[i] * w[i];
-        s[0] += a[k];
-        s[1] = fmaf(a[k], hat[k], s[1]);
-      }
-      if (p.h) {
-        c.load8(static_cast<const T*>(p.b), g, d);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = fmaf(hat[g * 8 + i], w[i], d[i]);
-        c.store8(static_cast<T*>(p.h) + row * p.cols, g, d);
-      }
-    }
-    block_sums(s, sh);
-    const float s0 = s[0] / p.cols, s1 = s[1] / p.cols;
-    s[0] = s[1] = 0.f;
-#pragma unroll
-    for (int g = 0; g < NV; ++g) {
-      float d[8];
-      if (p.du) {
-        get_t(p.du, p.ld_du, R::kDu, g, d);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = g * 8 + i;
-        a[k] = fmaf(rstd_u, a[k] - fmaf(hat[k], s1, s0), d[i]);
-        d[i] = p.alpha * a[k];
-      }
-      c.store8(static_cast<T*>(p.dx) + row * p.ld_dx, g, d);
-      if constexpr (BRANCH) {
-        float w[8];
-        get_kept(p.y, p.ld_y, R::kY, R::kUnitY, g, hat + g * 8);
-        c.load8(static_cast<const T*>(p.pw), g, w);
-        c.load8(static_cast<const T*>(p.gate), g, d);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = g * 8 + i;
-          hat[k] = (hat[k] - mean_y) * rstd_y;
-          P[k] = fmaf(a[k], hat[k], P[k]);
-          Q[k] += a[k];
-          a[k] *= d[i] * w[i];
-          s[0] += a[k];
-          s[1] = fmaf(a[k], hat[k], s[1]);
-        }
-      }
-    }
-    if constexpr (BRANCH) {
-      block_sums(s, sh + 2);
-      const float t0 = s[0] / p.cols, t1 = s[1] / p.cols;
 #pragma unroll
       for (int g = 0; g < NV; ++g) {
-        float d[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = rstd_y * (a[g * 8 + i] - fmaf(hat[g * 8 + i], t1, t0));
-        c.store8(static_cast<T*>(p.dy) + row * p.ld_dy, g, d);
+        const int col = C::column(g);
+        if (col >= cols) continue;
+        copy_async<8>(region + (g * NT + threadIdx.x) * 8, r + col);
+        copy_async<4>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4,
+                      r + pack_code_bytes(cols) + (col / kPackGroup & ~3));
       }
-    } else if (blockDim.x > 32) {
-      __syncthreads();  // sh is written again by the next row
+    } else {
+      for (int i = threadIdx.x; i < int(pack_row_bytes(cols)) / 16; i += NT) copy_async<16>(region + i * 16, r + i * 16);
     }
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
+  static __device__ __forceinline__ void get(const char* region, const Matrix&, int64_t, int cols, int g, Two* v) {
+    float f[8];
+    if constexpr (VEC) {
+      const int col = C::column(g);
+      uint2 codes = make_uint2(0, 0);
+      unsigned byte = 1;
+      if (col < cols) {
+        codes = *reinterpret_cast<const uint2*>(region + (g * NT + threadIdx.x) * 8);
+        const unsigned four = *reinterpret_cast<const unsigned*>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4);
+        byte = four >> (8 * (col / kPackGroup & 3)) & 0xffu;
+      }
+      decode8(codes, pack_unit(byte), f);
+    } else {
+      const unsigned char* r = reinterpret_cast<const unsigned char*>(region);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = C::column(g, i);
+        f[i] = col < cols ? decode1(r[col], pack_unit(r[pack_code_bytes(cols) + col / kPackGroup])) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+  }
+};
+
+// Walks over a CTA's rows with the next ones on their way: fetch(row, stage) starts
+// the copies of a row, work(row, stage) has them in place.
+template <int NT, bool VEC, int STAGES, typename Fetch, typename Work>
+__device__ __forceinline__ void walk(int rows, Fetch&& fetch, Work&& work) {
+  const int64_t step = gridDim.x;
+  if constexpr (STAGES == 1) {
+    for (int64_t row = blockIdx.x; row < rows; row += step) {
+      if constexpr (!VEC) __syncthreads();  // the last row has been read
+      fetch(row, 0);
+      copies_commit();
+      copies_wait<0>();
+      if constexpr (!VEC) __syncthreads();
+      work(row, 0);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      const int64_t row = blockIdx.x + s * step;
+      if (row < rows) fetch(row, s);
+      copies_commit();
+    }
+    int stage = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += step) {
+      copies_wait<STAGES - 2>();
+      // Other threads' copies are in place, and the stage filled next has been read by all.
+      if constexpr (!VEC) __syncthreads();
+      const int64_t ahead = row + (STAGES - 1) * step;
+      if (ahead < rows) fetch(ahead, stage == 0 ? STAGES - 1 : stage - 1);
+      copies_commit();
+      work(row, stage);
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ forward
+struct JoinFwd {
+  Matrix x, y;
+  const void *pw, *pb, *gate, *w, *b;
+  void *u, *h;
+  float* stats;  // [4][rows]: mean_y, rstd_y, mean_u, rstd_u
+  int64_t ld_h;
+  int rows, cols;
+  float alpha, eps, inverse;  // inverse: 1 / cols
+};
+
+// Mean and reciprocal deviation of a row: two passes over registers.
+template <int NT, int NV, bool VEC, typename C>
+__device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, float* sh) {
+  Two s = 0;
+#pragma unroll
+  for (int i = 0; i < NV * 4; ++i) s = two_add(s, v[i]);
+  const float mean = cta_sum<NT>(total(s), sh) * p.inverse;
+  const Two minus = two(-mean, -mean);
+  s = 0;
+#pragma unroll
+  for (int g = 0; g < NV; ++g) {
+    Two q = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Two d = two_add(v[g * 4 + i], minus);
+      if (!VEC) {  // single columns may lie past the width
+        const float2 f = both(d);
+        d = two(C::column(g, 2 * i) < p.cols ? f.x : 0.f, C::column(g, 2 * i + 1) < p.cols ? f.y : 0.f);
+      }
+      q = two_fma(d, d, q);
+    }
+    if (!VEC || C::column(g) < p.cols) s = two_add(s, q);
+  }
+  const float var = cta_sum<NT>(total(s), sh + 16) * p.inverse;
+  return make_float2(mean, rsqrtf(var + p.eps));
+}
+
+template <typename T, int NT, int NV, bool VEC, int STAGES>
+__global__ void __launch_bounds__(NT) join_fwd_kernel(JoinFwd p) {
+  extern __shared__ __align__(16) char ring[];
+  __shared__ __align__(16) float sh[64];
+  using C = Tile<T, NT, NV, VEC>;
+  const int bytes = C::bytes(p.cols);
+  walk<NT, VEC, STAGES>(
+      p.rows,
+      [&](int64_t row, int stage) {
+        C::fetch(ring + (2 * stage) * bytes, p.y, row, p.rows, p.cols);
+        C::fetch(ring + (2 * stage + 1) * bytes, p.x, row, p.rows, p.cols);
+      },
+      [&](int64_t row, int stage) {
+        Two y[NV * 4];
+#pragma unroll
+        for (int g = 0; g < NV; ++g) C::get(ring + (2 * stage) * bytes, p.y, row, p.cols, g, y + g * 4);
+        float2 st = row_stats<NT, NV, VEC, C>(y, p, sh);
+        if (threadIdx.x == 0) {
+          p.stats[row] = st.x;
+          p.stats[p.rows + row] = st.y;
+        }
+        Two scale = two(st.y, st.y), minus = two(-st.x, -st.x);
+        const Two alpha = two(p.alpha, p.alpha);
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+          Two w[4], b[4], v[4];
+          C::vector(p.pw, p.cols, g, w);
+          C::vector(p.pb, p.cols, g, b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[g * 4 + i] = two_fma(two_mul(two_add(y[g * 4 + i], minus), scale), w[i], b[i]);
+          C::vector(p.gate, p.cols, g, w);
+          C::get(ring + (2 * stage + 1) * bytes, p.x, row, p.cols, g, v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[g * 4 + i] = two_fma(w[i], y[g * 4 + i], two_mul(alpha, v[i]));
+          C::store(p.u, p.cols, row, p.cols, g, y + g * 4);
+        }
+        st = row_stats<NT, NV, VEC, C>(y, p, sh + 32);
+        if (threadIdx.x == 0) {
+          p.stats[2 * int64_t(p.rows) + row] = st.x;
+          p.stats[3 * int64_t(p.rows) + row] = st.y;
+        }
+        scale = two(st.y, st.y), minus = two(-st.x, -st.x);
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+          Two w[4], b[4];
+          C::vector(p.w, p.cols, g, w);
+          C::vector(p.b, p.cols, g, b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[i] = two_fma(two_mul(two_add(y[g * 4 + i], minus), scale), w[i], b[i]);
+          C::store(p.h, p.ld_h, row, p.cols, g, b);
+        }
+      });
+}
+
+// ----------------------------------------------------------------- backward
+struct JoinBwd {
+  Matrix dh, du, u, y;  // du.data may be null; u and y rows may be packed
+  const void *pw, *gate, *w, *b;  // b: only for h
+  const float *mean_y, *rstd_y, *mean_u, *rstd_u;
+  void *dx, *dy, *h;  // h (optional): the norm's output again
+  float* sums;        // [grid][2 or 4][cols]
+  int64_t ld_dy, ld_dx;
+  int rows, cols;
+  float alpha, inverse;
+};
+
+template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
+struct BwdTiles {
+  using C = Tile<T, NT, NV, VEC>;
+  using K = std::conditional_t<PACKED, PackedTile<NT, NV, VEC>, C>;
+  static __host__ __device__ constexpr int bytes(int cols) { return 2 * C::bytes(cols) + (BRANCH ? 2 : 1) * K::bytes(cols); }
+};
+
+// A row takes two CTA-wide reductions (one without a branch), the second one of
+// values that the first decides.  The column sums stay in registers: 64 of them for
+// sixteen columns a thread, which is what limits an SM to 512 threads.
+template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
+__global__ void __launch_bounds__(NT, 512 / NT) join_bwd_kernel(JoinBwd p) {
+  constexpr int N = NV * 4;
+  extern __shared__ __align__(16) char ring[];
+  __shared__ __align__(16) float2 sh[2][16];
+  using Tiles = BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>;
+  using C = typename Tiles::C;
+  using K = typename Tiles::K;
+  const int whole = C::bytes(p.cols), kept = K::bytes(p.cols), bytes = Tiles::bytes(p.cols);
+  Two dw[N], db[N], P[BRANCH ? N : 1], Q[BRANCH ? N : 1];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    dw[i] = db[i] = 0;
+    if (BRANCH) P[i] = Q[i] = 0;
+  }
+  int turn = 0;  // without a branch: the reductions' buffers alternate
+  walk<NT, VEC, STAGES>(
+      p.rows,
+      [&](int64_t row, int stage) {
+        char* r = ring + stage * bytes;
+        C::fetch(r, p.dh, row, p.rows, p.cols);
+        K::fetch(r + 2 * whole, p.u, row, p.rows, p.cols);
+        if (p.du.data) C::fetch(r + whole, p.du, row, p.rows, p.cols);
+        if (BRANCH) K::fetch(r + 2 * whole + kept, p.y, row, p.rows, p.cols);
+      },
+      [&](int64_t row, int stage) {
+        const char* r = ring + stage * bytes;
+        const float mean_u = p.mean_u[row], rstd_u = p.rstd_u[row];
+        float mean_y = 0.f, rstd_y = 0.f;
+        if (BRANCH) {
+          mean_y = p.mean_y[row];
+          rstd_y = p.rstd_y[row];
+        }
+        Two hat[N], a[N], s0 = 0, s1 = 0;
+        {
+          const Two scale = two(rstd_u, rstd_u), minus = two(-mean_u, -mean_u);
+#pragma unroll
+          for (int g = 0; g < NV; ++g) {
+            Two d[4], w[4];
+            C::get(r, p.dh, row, p.cols, g, d);
+            K::get(r + 2 * whole, p.u, row, p.cols, g, hat + g * 4);
+            C::vector(p.w, p.cols, g, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = g * 4 + i;
+              hat[k] = two_mul(two_add(hat[k], minus), scale);
+              dw[k] = two_fma(d[i], hat[k], dw[k]);
+              db[k] = two_add(db[k], d[i]);
+              a[k] = two_mul(d[i], w[i]);
+              s0 = two_add(s0, a[k]);
+              s1 = two_fma(a[k], hat[k], s1);
+            }
+            if (p.h) {
+              C::vector(p.b, p.cols, g, d);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) d[i] = two_fma(hat[g * 4 + i], w[i], d[i]);
+              C::store(p.h, p.cols, row, p.cols, g, d);
+            }
+          }
+        }
+        float2 m = cta_sum2<NT>(total(s0), total(s1), sh[BRANCH ? 0 : turn]);
+        turn ^= 1;
+        {
+          // dt = du + rstd (a - <a> - hat <a hat>)
+          const Two m0 = two(-m.x * p.inverse, -m.x * p.inverse), m1 = two(-m.y * p.inverse, -m.y * p.inverse);
+          const Two rstd = two(rstd_u, rstd_u), alpha = two(p.alpha, p.alpha);
+          const Two scale = two(rstd_y, rstd_y), minus = two(-mean_y, -mean_y);
+          s0 = s1 = 0;
+#pragma unroll
+          for (int g = 0; g < NV; ++g) {
+            Two d[4] = {0, 0, 0, 0};
+            if (p.du.data) C::get(r + whole, p.du, row, p.cols, g, d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = g * 4 + i;
+              a[k] = two_fma(two_add(a[k], two_fma(hat[k], m1, m0)), rstd, d[i]);
+              d[i] = two_mul(alpha, a[k]);
+            }
+            C::store(p.dx, p.ld_dx, row, p.cols, g, d);
+            if constexpr (BRANCH) {
+              Two w[4];
+              K::get(r + 2 * whole + kept, p.y, row, p.cols, g, hat + g * 4);
+              C::vector(p.pw, p.cols, g, w);
+              C::vector(p.gate, p.cols, g, d);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = g * 4 + i;
+                hat[k] = two_mul(two_add(hat[k], minus), scale);
+                P[k] = two_fma(a[k], hat[k], P[k]);
+                Q[k] = two_add(Q[k], a[k]);
+                a[k] = two_mul(a[k], two_mul(d[i], w[i]));
+                s0 = two_add(s0, a[k]);
+                s1 = two_fma(a[k], hat[k], s1);
+              }
+            }
+          }
+        }
+        if constexpr (BRANCH) {
+          m = cta_sum2<NT>(total(s0), total(s1), sh[1]);
+          const Two m0 = two(-m.x * p.inverse, -m.x * p.inverse), m1 = two(-m.y * p.inverse, -m.y * p.inverse);
+          const Two rstd = two(rstd_y, rstd_y);
+#pragma unroll
+          for (int g = 0; g < NV; ++g) {
+            Two d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = two_mul(two_add(a[g * 4 + i], two_fma(hat[g * 4 + i], m1, m0)), rstd);
+            C::store(p.dy, p.ld_dy, row, p.cols, g, d);
+          }
+        }
+      });
+  using F = Tile<float, NT, NV, VEC>;
   float* out = p.sums + int64_t(blockIdx.x) * (BRANCH ? 4 : 2) * p.cols;
 #pragma unroll
   for (int g = 0; g < NV; ++g) {
-    c.store8(out, g, dw + g * 8);
-    c.store8(out + p.cols, g, db + g * 8);
+    F::store(out, 0, 0, p.cols, g, dw + g * 4);
+    F::store(out + p.cols, 0, 0, p.cols, g, db + g * 4);
     if constexpr (BRANCH) {
-      c.store8(out + 2 * int64_t(p.cols), g, P + g * 8);
-      c.store8(out + 3 * int64_t(p.cols), g, Q + g * 8);
+      F::store(out + 2 * int64_t(p.cols), 0, 0, p.cols, g, P + g * 4);
+      F::store(out + 3 * int64_t(p.cols), 0, 0, p.cols, g, Q + g * 4);
     }
   }
 }
@@ -435,16 +565,17 @@ struct JoinFinish {
   int parts, cols;
 };
 
-// 32 columns a CTA; each of its 8 rows of threads adds every eighth partial sum.
+// 32 columns a CTA; each of its 32 warps adds every 32nd partial sum, in order.
 template <typename T, bool BRANCH>
-__global__ void __launch_bounds__(256) join_finish_kernel(JoinFinish p) {
+__global__ void __launch_bounds__(1024) join_finish_kernel(JoinFinish p) {
   constexpr int K = BRANCH ? 4 : 2;
-  __shared__ float sh[K][8][32];
+  __shared__ float sh[K][32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane;
   float s[K] = {};
   if (col < p.cols) {
-    for (int q = part; q < p.parts; q += 8) {
+#pragma unroll 4
+    for (int q = part; q < p.parts; q += 32) {
 #pragma unroll
       for (int k = 0; k < K; ++k) s[k] += p.sums[(int64_t(q) * K + k) * p.cols + col];
     }
@@ -452,44 +583,31 @@ __global__ void __launch_bounds__(256) join_finish_kernel(JoinFinish p) {
 #pragma unroll
   for (int k = 0; k < K; ++k) sh[k][part][lane] = s[k];
   __syncthreads();
-  if (part || col >= p.cols) return;
+  // Warp k sums the k-th column sum of the 32 columns; warp 0 writes.
+  if (part < K) {
+    float v = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    s[k] = 0.f;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) s[k] += sh[k][q][lane];
+    for (int q = 0; q < 32; ++q) v += sh[part][q][lane];
+    sh[part][0][lane] = v;
   }
-  static_cast<T*>(p.dw)[col] = from_float<T>(s[0]);
-  static_cast<T*>(p.db)[col] = from_float<T>(s[1]);
+  __syncthreads();
+  if (part || col >= p.cols) return;
+  static_cast<T*>(p.dw)[col] = from_float<T>(sh[0][0][lane]);
+  static_cast<T*>(p.db)[col] = from_float<T>(sh[1][0][lane]);
   if constexpr (BRANCH) {
     const float pw = to_float(static_cast<const T*>(p.pw)[col]), pb = to_float(static_cast<const T*>(p.pb)[col]);
     const float g = to_float(static_cast<const T*>(p.gate)[col]);
-    static_cast<T*>(p.dgate)[col] = from_float<T>(pw * s[2] + pb * s[3]);
-    static_cast<T*>(p.dpw)[col] = from_float<T>(g * s[2]);
-    static_cast<T*>(p.dpb)[col] = from_float<T>(g * s[3]);
+    static_cast<T*>(p.dgate)[col] = from_float<T>(pw * sh[2][0][lane] + pb * sh[3][0][lane]);
+    static_cast<T*>(p.dpw)[col] = from_float<T>(g * sh[2][0][lane]);
+    static_cast<T*>(p.dpb)[col] = from_float<T>(g * sh[3][0][lane]);
   }
 }
 
-// Groups of eight columns a thread has: enough work per thread that the reductions
-// over the CTA weigh little, few enough registers that several CTAs share an SM.
-int fwd_groups(int64_t cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : 4; }
-int bwd_groups(int64_t cols) { return cols <= 1024 ? 1 : 2; }
-int threads_for(int64_t cols, int nv) { return int((cols + nv * 8 - 1) / (nv * 8) + 31) / 32 * 32; }
-
-template <typename T>
-int fwd_typed(const JoinFwd& p, bool vec, cudaStream_t s) {
-  const int nv = fwd_groups(p.cols);
-  auto launch = [&](auto kernel) { kernel<<<unsigned(p.rows), threads_for(p.cols, nv), 0, s>>>(p); };
-  if (nv == 1) vec ? launch(join_fwd_kernel<T, 1, true>) : launch(join_fwd_kernel<T, 1, false>);
-  else if (nv == 2) vec ? launch(join_fwd_kernel<T, 2, true>) : launch(join_fwd_kernel<T, 2, false>);
-  else vec ? launch(join_fwd_kernel<T, 4, true>) : launch(join_fwd_kernel<T, 4, false>);
-  return int(cudaGetLastError());
-}
-
+// -------------------------------------------------------------------- launches
 // Shared memory above 48 KB (the kernel's fixed part counts too), once for each kernel and device.
 template <auto Kernel>
 int opt_in(int smem) {
-  if (smem <= 47 * 1024) return 0;
+  if (smem <= 40 * 1024) return 0;
   static std::atomic<uint64_t> opted{0};
   int device = 0;
   cudaGetDevice(&device);
@@ -499,55 +617,73 @@ int opt_in(int smem) {
   if (e == cudaSuccess) opted.fetch_or(bit, std::memory_order_relaxed);
   return int(e);
 }
-
-template <typename T, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
-int bwd_launch(const JoinBwd& p, int parts, cudaStream_t s) {
-  constexpr auto kernel = join_bwd_kernel<T, NV, VEC, BRANCH, PACKED, STAGES>;
-  const int threads = threads_for(p.cols, NV);
-  const int smem = VEC ? Ring<T, NV, BRANCH, PACKED, STAGES>::bytes(threads) : 0;
-  if (const int r = opt_in<join_bwd_kernel<T, NV, VEC, BRANCH, PACKED, STAGES>>(smem)) return r;
-  kernel<<<unsigned(parts), threads, smem, s>>>(p);
-  return int(cudaGetLastError());
+// CTAs of 512 / NT or what the rings leave room for, on every SM.
+int most_ctas(int nt, int ring) {
+  const int fit = kMaxRing / (ring > 0 ? ring : 1);
+  const int by_threads = 512 / nt;
+  return 148 * (fit < by_threads ? (fit < 1 ? 1 : fit) : by_threads);
 }
 
-template <typename T, int NV, bool BRANCH, bool PACKED>
-int bwd_pick(const JoinBwd& p, int parts, bool vec, cudaStream_t s) {
-  if (!vec) return bwd_launch<T, NV, false, BRANCH, PACKED, 1>(p, parts, s);
-  if (Ring<T, NV, BRANCH, PACKED, 3>::bytes(threads_for(p.cols, NV)) <= kMaxRing)
-    return bwd_launch<T, NV, true, BRANCH, PACKED, 3>(p, parts, s);
-  return bwd_launch<T, NV, true, BRANCH, PACKED, 1>(p, parts, s);
+template <typename T, int NT, int NV, bool VEC>
+int fwd_launch(const JoinFwd& p, cudaStream_t s) {
+  const int smem = kStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
+  if (smem > kMaxRing) return -1;
+  if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kStages>>(smem)) return r;
+  join_fwd_kernel<T, NT, NV, VEC, kStages><<<unsigned(std::min(p.rows, most_ctas(NT, smem))), NT, smem, s>>>(p);
+  return int(cudaGetLastError());
+}
+template <typename T, bool VEC>
+int fwd_pick(const JoinFwd& p, cudaStream_t s) {
+  if (p.cols <= 256) return fwd_launch<T, 32, 1, VEC>(p, s);
+  if (p.cols <= 1024) return fwd_launch<T, 128, 1, VEC>(p, s);
+  if (p.cols <= 2048) return fwd_launch<T, 128, 2, VEC>(p, s);
+  if (p.cols <= 4096) return fwd_launch<T, 128, 4, VEC>(p, s);
+  return fwd_launch<T, 256, 4, VEC>(p, s);
 }
 
-template <typename T, bool BRANCH, bool PACKED>
-int bwd_typed(const JoinBwd& p, const JoinFinish& f, int parts, bool vec, cudaStream_t s) {
-  const int r = bwd_groups(p.cols) == 1 ? bwd_pick<T, 1, BRANCH, PACKED>(p, parts, vec, s)
-                                        : bwd_pick<T, 2, BRANCH, PACKED>(p, parts, vec, s);
-  if (r) return r;
-  join_finish_kernel<T, BRANCH><<<unsigned((p.cols + 31) / 32), 256, 0, s>>>(f);
+// The gradient's CTAs: as many as fit, but four rows each where that leaves every SM one.
+template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
+int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
+  // Three rows of the widest FP32 tensors are more than an SM holds.
+  constexpr int kRows = sizeof(T) == 4 && NT == 512 ? 1 : kStages;
+  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols);
+  if (smem > kMaxRing) return -1;
+  if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
+  f.parts = std::min(std::min(p.rows, most_ctas(NT, smem)), std::max(p.rows / 4, 148));
+  join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
+  if (const int r = int(cudaGetLastError())) return r;
+  join_finish_kernel<T, BRANCH><<<unsigned((p.cols + 31) / 32), 1024, 0, s>>>(f);
   return int(cudaGetLastError());
+}
+template <typename T, bool VEC, bool BRANCH, bool PACKED>
+int bwd_pick(const JoinBwd& p, const JoinFinish& f, cudaStream_t s) {
+  if (p.cols <= 256) return bwd_launch<T, 32, 1, VEC, BRANCH, PACKED>(p, f, s);
+  if (p.cols <= 1024) return bwd_launch<T, 128, 1, VEC, BRANCH, PACKED>(p, f, s);
+  if (p.cols <= 2048) return bwd_launch<T, 128, 2, VEC, BRANCH, PACKED>(p, f, s);
+  if (p.cols <= 4096) return bwd_launch<T, 256, 2, VEC, BRANCH, PACKED>(p, f, s);
+  return bwd_launch<T, 512, 2, VEC, BRANCH, PACKED>(p, f, s);
 }
 }  // namespace
 
 int64_t join_max_cols() { return kJoinMaxCols; }
 int join_bwd_parts(int64_t rows, int64_t cols) {
-  // CTAs that fit the GPU at once by registers (128 a thread) and, at most, four an SM.
-  const int threads = threads_for(cols, bwd_groups(cols));
-  const int per_sm = threads >= 512 ? 1 : threads >= 256 ? 2 : 4;
-  const int64_t most = 148 * per_sm;
-  return int(rows < most ? rows : most);
+  // The most that any form launches at this width (threads alone).
+  const int nt = cols <= 256 ? 32 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  return int(std::min<int64_t>(rows, 148 * (512 / nt)));
 }
 
 int join_fwd(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int type, const void* pw, const void* pb,
              const void* gate, const void* w, const void* b, void* u, void* h, int64_t ld_h, float* stats, int64_t rows,
              int64_t cols, float alpha, float eps, cudaStream_t s) {
   if (rows <= 0 || rows > 0x7fffffff || cols <= 0 || cols > kJoinMaxCols) return -1;
-  const JoinFwd p{x, y, pw, pb, gate, w, b, u, h, stats, ld_x, ld_y, ld_h, int(rows), int(cols), alpha, eps};
+  const JoinFwd p{{x, ld_x}, {y, ld_y}, pw, pb, gate, w, b, u, h, stats, ld_h, int(rows), int(cols), alpha, eps,
+                  1.f / float(cols)};
   const int64_t size = type == kTypeFP32 ? 4 : 2;
   const bool vec = cols % 8 == 0 && ld_x * size % 16 == 0 && ld_y * size % 16 == 0 && ld_h * size % 16 == 0 &&
                    aligned16(x) && aligned16(y) && aligned16(pw) && aligned16(pb) && aligned16(gate) && aligned16(w) &&
                    aligned16(b) && aligned16(u) && aligned16(h);
-  if (type == kTypeBF16) return fwd_typed<__nv_bfloat16>(p, vec, s);
-  if (type == kTypeFP32) return fwd_typed<float>(p, vec, s);
+  if (type == kTypeBF16) return vec ? fwd_pick<__nv_bfloat16, true>(p, s) : fwd_pick<__nv_bfloat16, false>(p, s);
+  if (type == kTypeFP32) return vec ? fwd_pick<float, true>(p, s) : fwd_pick<float, false>(p, s);
   return -1;
 }
 
@@ -555,10 +691,10 @@ int join_bwd(const JoinBwdCall& c, cudaStream_t s) {
   if (c.rows <= 0 || c.rows > 0x7fffffff || c.cols <= 0 || c.cols > kJoinMaxCols) return -1;
   const bool branch = c.y != nullptr;
   if (!branch && !c.packed) return -1;
-  const int parts = join_bwd_parts(c.rows, c.cols);
-  const JoinBwd p{c.dh, c.du, c.u, c.y, c.pw, c.gate, c.w, c.b, c.mean_y, c.rstd_y, c.mean_u, c.rstd_u, c.dx, c.dy, c.h, c.workspace,
-                  c.ld_dh, c.ld_du, c.ld_u, c.ld_y, c.ld_dy, c.ld_dx, int(c.rows), int(c.cols), c.alpha};
-  const JoinFinish f{c.workspace, c.pw, c.pb, c.gate, c.dw, c.db, c.dpw, c.dpb, c.dgate, parts, int(c.cols)};
+  const JoinBwd p{{c.dh, c.ld_dh}, {c.du, c.ld_du}, {c.u, c.ld_u}, {c.y, c.ld_y}, c.pw, c.gate, c.w, c.b,
+                  c.mean_y, c.rstd_y, c.mean_u, c.rstd_u, c.dx, c.dy, c.h, c.workspace, c.ld_dy, c.ld_dx,
+                  int(c.rows), int(c.cols), c.alpha, 1.f / float(c.cols)};
+  const JoinFinish f{c.workspace, c.pw, c.pb, c.gate, c.dw, c.db, c.dpw, c.dpb, c.dgate, 0, int(c.cols)};
   const int64_t size = c.type == kTypeFP32 ? 4 : 2;
   auto fine = [&](const void* q, int64_t ld) { return !q || (aligned16(q) && ld * size % 16 == 0); };
   const bool vec = c.cols % 8 == 0 && fine(c.dh, c.ld_dh) && fine(c.du, c.ld_du) && fine(c.dx, c.ld_dx) &&
@@ -567,8 +703,9 @@ int join_bwd(const JoinBwdCall& c, cudaStream_t s) {
                    (c.packed || (fine(c.u, c.ld_u) && fine(c.y, c.ld_y)));
   auto pick = [&](auto zero) {
     using T = decltype(zero);
-    if (!branch) return bwd_typed<T, false, true>(p, f, parts, vec, s);
-    return c.packed ? bwd_typed<T, true, true>(p, f, parts, vec, s) : bwd_typed<T, true, false>(p, f, parts, vec, s);
+    if (!branch) return vec ? bwd_pick<T, true, false, true>(p, f, s) : bwd_pick<T, false, false, true>(p, f, s);
+    if (c.packed) return vec ? bwd_pick<T, true, true, true>(p, f, s) : bwd_pick<T, false, true, true>(p, f, s);
+    return vec ? bwd_pick<T, true, true, false>(p, f, s) : bwd_pick<T, false, true, false>(p, f, s);
   };
   if (c.type == kTypeBF16) return pick(__nv_bfloat16());
   if (c.type == kTypeFP32) return pick(float());

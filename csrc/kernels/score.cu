@@ -9,7 +9,7 @@
 // Forward: a cluster of 1 to 8 CTAs per row, each thread with running (m, s, u)
 // in FP32 over 16-byte vectors; a logit of -inf adds nothing.  The alternatives
 // need no sort of the row: each thread keeps its largest value and the start of
-// the vector that held it.  The k-th largest of these 256 (value, start) pairs
+// the vector that held it.  The k-th largest of these (value, start) pairs
 // bounds the k-th largest logit from below, and only the k threads at or above
 // it can hold one, so a second look at those threads' vectors collects the few
 // candidates, which one warp sorts.  Equal values go to the lowest index.
@@ -28,7 +28,7 @@ namespace cg = cooperative_groups;
 namespace tn5b {
 namespace kernels {
 namespace {
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;  // of the merge and the gradient
 constexpr int kMaxTop = 32;       // alternatives a row: one sorted list per warp
 constexpr int kCandidates = 1024;  // 8 KB; more than that takes the selection by rounds
 constexpr int kUnroll = 4;
@@ -342,25 +342,28 @@ struct Part {
   __device__ __forceinline__ unsigned vector_at(unsigned j) const { return head + j * Vec<T>::kN; }
 };
 
+template <int NT>
 struct TopShared {
-  Key lists[kWarps][32];
+  static constexpr int W = NT / 32;
+  Key lists[W][32];
   Key candidates[kCandidates];
-  Key best[kWarps];
-  unsigned active[kThreads];
+  Key best[W];
+  unsigned active[NT];
   unsigned active_count, count;
 };
 
 // Descending list of the CTA's 32 best, of which the first k count, in every
 // lane of warp 0 (and in sh.lists[0]).
-template <typename T>
-__device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, TopShared& sh) {
+template <typename T, int NT>
+__device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, TopShared<NT>& sh) {
+  constexpr int W = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) sh.active_count = sh.count = 0;
   Key list = sort_warp(own);
   sh.lists[warp][lane] = list;
   __syncthreads();
 #pragma unroll
-  for (int half = kWarps / 2; half; half >>= 1) {
+  for (int half = W / 2; half; half >>= 1) {
     if (warp < half) {
       list = merge_warp(list, sh.lists[warp + half][lane]);
       sh.lists[warp][lane] = list;
@@ -373,13 +376,13 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
 
   // Visits every value whose (value, start of vector) reaches the bound; its own
   // key is handed on.  Items: the active threads' vectors, then single values.
-  const unsigned per = (part.vectors + kThreads - 1) / kThreads;
+  const unsigned per = (part.vectors + NT - 1) / NT;
   const unsigned scalars = part.head + part.tail;
   const unsigned items = sh.active_count * per;
   auto visit = [&](auto&& take) {
-    for (unsigned i = tid; i < items + scalars; i += kThreads) {
+    for (unsigned i = tid; i < items + scalars; i += NT) {
       if (i < items) {
-        const unsigned a = i / per, j = sh.active[a] + (i - a * per) * kThreads;
+        const unsigned a = i / per, j = sh.active[a] + (i - a * per) * NT;
         if (j >= part.vectors) continue;
         const unsigned at = part.vector_at(j);
         Vec<T> vec;
@@ -429,7 +432,7 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
       __syncthreads();
       best = sh.best[0];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) best = best > sh.best[w] ? best : sh.best[w];
+      for (int w = 1; w < W; ++w) best = best > sh.best[w] ? best : sh.best[w];
       below = best;
       if (tid == 0) sh.lists[0][r] = best;
       __syncthreads();
@@ -440,13 +443,14 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
 }
 
 // grid = rows * C CTAs in clusters of C; the cluster's CTAs take `chunk` columns each.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_t ld, unsigned vocab,
+template <typename T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT) score_kernel(const T* logits, int64_t ld, unsigned vocab,
                                                          const int64_t* targets, int64_t start,
                                                          int64_t vocab_total, unsigned chunk, Out o) {
-  __shared__ Sums warp_sums[kWarps];
+  constexpr int W = NT / 32;
+  __shared__ Sums warp_sums[W];
   __shared__ Sums block_sums;
-  __shared__ std::conditional_t<TOP, TopShared, int> sh;
+  __shared__ std::conditional_t<TOP, TopShared<NT>, int> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
   const int row = blockIdx.x / C;
@@ -464,13 +468,13 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_
     if (unsigned(tid) < part.head) run.add_one(to_float(part.x[tid]), part.lo + tid);
     const uint4* vectors = reinterpret_cast<const uint4*>(part.x + part.head);
     unsigned j = tid;
-    for (; j + (kUnroll - 1) * kThreads < part.vectors; j += kUnroll * kThreads) {
+    for (; j + (kUnroll - 1) * NT < part.vectors; j += kUnroll * NT) {
       uint4 raw[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) raw[i] = vectors[j + i * kThreads];
-      run.template add<kUnroll>(raw, part.lo + part.vector_at(j), kThreads * kN);
+      for (int i = 0; i < kUnroll; ++i) raw[i] = vectors[j + i * NT];
+      run.template add<kUnroll>(raw, part.lo + part.vector_at(j), NT * kN);
     }
-    for (; j < part.vectors; j += kThreads) {
+    for (; j < part.vectors; j += NT) {
       const uint4 raw = vectors[j];
       run.template add<1>(&raw, part.lo + part.vector_at(j), 0);
     }
@@ -485,13 +489,13 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_
   __syncthreads();
   float top = warp_sums[0].m;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) top = max_nan(top, warp_sums[w].m);
+  for (int w = 1; w < W; ++w) top = max_nan(top, warp_sums[w].m);
   const bool plain = top > plain_low<T>() && top < kPlain;
   if (plain) {
     if (tid == 0) {
       Sums a{top, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float d = reference(warp_sums[w].m) - reference(top), f = fast_exp2(d);
         a.s += warp_sums[w].s * f;
         a.u += (warp_sums[w].u + d * warp_sums[w].s) * f;
@@ -504,7 +508,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_
       const float v = to_float(part.x[tid]);
       run.template add<1>(&v, part.lo + tid);
     }
-    for (unsigned j = tid; j < part.vectors; j += kThreads) {
+    for (unsigned j = tid; j < part.vectors; j += NT) {
       Vec<T> vec;
       float v[kN];
       vec.load(part.x + part.vector_at(j));
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const T* logits, int64_
     if (tid == 0) {
       a = warp_sums[0];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) a = join(a, warp_sums[w]);
+      for (int w = 1; w < W; ++w) a = join(a, warp_sums[w]);
       block_sums = a;
     }
     if (TOP) key = run.key();
@@ -659,17 +663,14 @@ __global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, in
   }
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int NT>
 int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
-                 int64_t vocab_total, const Out& o, cudaStream_t s) {
-  // A row is split over a cluster while the rows alone leave SMs idle.
-  unsigned C = 1;
-  while (C < 8 && int64_t(o.rows) * C * 2 <= 148 * 4 && vocab / (2 * C) >= 4096) C *= 2;
+                 int64_t vocab_total, const Out& o, unsigned C, cudaStream_t s) {
   const unsigned step = Vec<T>::kN;  // every part is off a 16-byte boundary by what the row is
   const unsigned chunk = C == 1 ? vocab : ((vocab + C - 1) / C + step - 1) / step * step;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(o.rows) * C);
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(NT);
   config.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -677,14 +678,19 @@ int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&config, score_kernel<T, TOP>, static_cast<const T*>(logits), ld, vocab, targets,
+  return int(cudaLaunchKernelEx(&config, score_kernel<T, TOP, NT>, static_cast<const T*>(logits), ld, vocab, targets,
                                 start, vocab_total, chunk, o));
 }
+// Threads of a row's CTA, and CTAs an SM takes at once.
+constexpr int kRowThreads = 128, kRowCtas = 8;
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
-  return o.k ? launch_score<T, true>(logits, ld, vocab, targets, start, vocab_total, o, s)
-             : launch_score<T, false>(logits, ld, vocab, targets, start, vocab_total, o, s);
+  // A row is split over a cluster while the rows alone leave SMs idle.
+  unsigned C = 1;
+  while (C < 8 && int64_t(o.rows) * C * 2 <= 148 * kRowCtas && vocab / (2 * C) >= 4096) C *= 2;
+  return o.k ? launch_score<T, true, kRowThreads>(logits, ld, vocab, targets, start, vocab_total, o, C, s)
+             : launch_score<T, false, kRowThreads>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
 }
 template <typename T>
 int score_bwd_typed(const void* logits, int64_t ld, int rows, unsigned vocab, const int64_t* targets, int64_t start,
