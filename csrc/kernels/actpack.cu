@@ -201,78 +201,70 @@ __device__ __forceinline__ float kept_gelu(float v, const float* table) {
   return v * table[(kTablePad + k + int(bits >> 31) * kTableHalf) * kCopies];
 }
 
-// Sixteen columns per thread and step (one 16-byte load of codes), two steps at once.
+// Eight columns per thread and step; the next step's codes are loaded ahead.
 template <typename T, bool GELU>
-__global__ void __launch_bounds__(256) unpack_kernel(const unsigned char* data, T* out, T* act, int cols,
-                                                     unsigned segments, unsigned items) {
-  __shared__ __align__(16) float table[GELU ? kTableSize * kCopies : 4];
-  const int64_t row_bytes = pack_row_bytes(cols);
-  const int code_bytes = int(pack_code_bytes(cols));
-  const unsigned stride = gridDim.x * 256u;
-  constexpr int kSteps = 2;
-  bool ready = !GELU;
-  for (unsigned first = blockIdx.x * 256u + threadIdx.x; first < items || !ready; first += kSteps * stride) {
-    uint4 codes[kSteps];
-    unsigned byte[kSteps], row[kSteps];
-    int col[kSteps];
+__global__ void __launch_bounds__(1024, 2) unpack_kernel(const unsigned char* data, T* out, T* act, int cols,
+                                                         unsigned segments, unsigned items) {
+  extern __shared__ __align__(16) float table[];
+  const unsigned row_bytes = unsigned(pack_row_bytes(cols)), code_bytes = unsigned(pack_code_bytes(cols));
+  const unsigned stride = gridDim.x * 1024u, row_step = stride / segments, step = stride - row_step * segments;
+  unsigned item = blockIdx.x * 1024u + threadIdx.x;
+  unsigned row = item / segments, seg = item - row * segments;
+  uint2 codes = make_uint2(0, 0);
+  unsigned byte = 1;
+  auto load = [&] {
+    if (item < items) {
+      const unsigned char* src = data + int64_t(row) * row_bytes;
+      codes = *reinterpret_cast<const uint2*>(src + seg * 8);
+      byte = src[code_bytes + seg / (kPackGroup / 8)];
+    }
+  };
+  load();
+  if (GELU) {  // the table is filled while the first codes are on their way
+    fill_phi_table(table);
+    __syncthreads();
+  }
+  while (item < items) {
+    const uint2 now = codes;
+    const unsigned unit_byte = byte;
+    const int64_t at = int64_t(row) * cols + seg * 8;
+    item += stride;
+    row += row_step;
+    seg += step;
+    if (seg >= segments) {
+      seg -= segments;
+      ++row;
+    }
+    load();
+    const float unit = pack_unit(unit_byte);
+    // e in [-15, -1]: every code's binade lies in the table's window.
+    const bool window = unit_byte - 112u <= 14u;
+    const char* place = reinterpret_cast<const char*>(
+        table + (kTablePad + 8 * (int(unit_byte) - 127 + 9)) * kCopies + (threadIdx.x & (kCopies - 1)));
+    Two v[4], a[4];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const unsigned item = first + k * stride;
-      codes[k] = make_uint4(0, 0, 0, 0);
-      byte[k] = 1;
-      row[k] = item / segments;
-      col[k] = int(item - row[k] * segments) * 16;
-      if (item < items) {
-        const unsigned char* src = data + int64_t(row[k]) * row_bytes;
-        codes[k] = __ldcs(reinterpret_cast<const uint4*>(src + col[k]));
-        byte[k] = src[code_bytes + col[k] / kPackGroup];
+    for (int i = 0; i < 4; ++i) {
+      const unsigned word = i < 2 ? now.x : now.y;
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(i & 1 ? word >> 16 : word & 0xffffu), __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      v[i] = two_mul(two(f.x, f.y), two(unit, unit));
+      if (GELU && window) {
+        // Bits 7 .. 15 as an entry of 32 bytes: bits 5 .. 13 of the offset.
+        const unsigned w = unsigned(h.y) << 16 | h.x;
+        const float lo = *reinterpret_cast<const float*>(place + ((w >> 2) & 0x3fe0u));
+        const float hi = *reinterpret_cast<const float*>(place + ((w >> 18) & 0x3fe0u));
+        a[i] = two_mul(v[i], two(lo, hi));
       }
     }
-    if (!ready) {  // the table is filled while the first codes are on their way
-      fill_phi_table(table);
-      __syncthreads();
-      ready = true;
-    }
+    if (GELU && !window) {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      if (first + k * stride >= items) break;
-      const float unit = pack_unit(byte[k]);
-      const unsigned words[4] = {codes[k].x, codes[k].y, codes[k].z, codes[k].w};
-      // e in [-15, -1]: every code's binade lies in the table's window.
-      const bool window = byte[k] - 112u <= 14u;
-      const char* place = reinterpret_cast<const char*>(
-          table + (kTablePad + 8 * (int(byte[k]) - 127 + 9)) * kCopies + (threadIdx.x & (kCopies - 1)));
-      Two v[8], a[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const unsigned short code2 = i & 1 ? words[i / 2] >> 16 : words[i / 2] & 0xffffu;
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(code2), __NV_E4M3);
-        const float2 f = __half22float2(__half2(h));
-        v[i] = two_mul(two(f.x, f.y), two(unit, unit));
-        if (GELU && window) {
-          // Bits 7 .. 15 as an entry of 32 bytes: bits 5 .. 13 of the offset.
-          const unsigned w = unsigned(h.y) << 16 | h.x;
-          const float lo = *reinterpret_cast<const float*>(place + ((w >> 2) & 0x3fe0u));
-          const float hi = *reinterpret_cast<const float*>(place + ((w >> 18) & 0x3fe0u));
-          a[i] = two_mul(v[i], two(lo, hi));
-        }
-      }
-      if (GELU && !window) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 f = both(v[i]);
-          a[i] = two(kept_gelu(f.x, table), kept_gelu(f.y, table));
-        }
-      }
-      T* o = out + int64_t(row[k]) * cols + col[k];
-      T* g = act + int64_t(row[k]) * cols + col[k];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (col[k] + h * 8 >= cols) break;
-        put8(o + h * 8, v + h * 4);
-        if (GELU) put8(g + h * 8, a + h * 4);
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = both(v[i]);
+        a[i] = two(kept_gelu(f.x, table), kept_gelu(f.y, table));
       }
     }
+    put8(out + at, v);
+    if (GELU) put8(act + at, a);
   }
 }
 
@@ -326,15 +318,17 @@ int pack_typed(const void* x, int64_t ld, void* data, int64_t rows, int64_t cols
 template <typename T, bool GELU>
 int unpack_typed(const void* data, void* out, void* act, int64_t rows, int64_t cols, cudaStream_t s) {
   const bool vec = cols % 8 == 0 && aligned16(out) && (!GELU || aligned16(act));
-  const int64_t segments = vec ? (cols + 15) / 16 : (cols + 511) / 512, items = rows * segments;
+  const int64_t segments = vec ? cols / 8 : (cols + 511) / 512, items = rows * segments;
   if (items > 0x7fffffff) return -1;
-  const int64_t ctas = vec ? (items + 511) / 512 : (items + 7) / 8;
-  const unsigned grid = unsigned(ctas < 148 * 5 ? ctas : 148 * 5);  // five CTAs an SM: one table for many rows
-  auto launch = [&](auto kernel) {
-    kernel<<<grid, 256, 0, s>>>(static_cast<const unsigned char*>(data), static_cast<T*>(out), static_cast<T*>(act),
-                                int(cols), unsigned(segments), unsigned(items));
+  auto launch = [&](auto kernel, int per_cta, int threads, int most, int smem) {
+    const int64_t ctas = (items + per_cta - 1) / per_cta;
+    kernel<<<unsigned(ctas < most ? ctas : most), threads, smem, s>>>(
+        static_cast<const unsigned char*>(data), static_cast<T*>(out), static_cast<T*>(act), int(cols),
+        unsigned(segments), unsigned(items));
   };
-  vec ? launch(unpack_kernel<T, GELU>) : launch(unpack_odd_kernel<T, GELU>);
+  // Full SMs, and one table for many rows.
+  vec ? launch(unpack_kernel<T, GELU>, 1024, 1024, 148 * 2, GELU ? kTableSize * kCopies * 4 : 0)
+      : launch(unpack_odd_kernel<T, GELU>, 8, 256, 148 * 8, 0);
   return int(cudaGetLastError());
 }
 }  // namespace

@@ -38,7 +38,7 @@ namespace tn5b {
 namespace kernels {
 namespace {
 constexpr int kMaxRing = 200 * 1024;  // of an SM's 227 KB, for all CTAs on it
-constexpr int kStages = 3;
+constexpr int kFwdStages = 3, kBwdStages = 2;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -134,14 +134,20 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
+// A load that stays where it is written, before the barrier that follows.
+__device__ __forceinline__ uint4 ld_vector(const uint4* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
 // A [rows][cols] matrix with a row stride in elements (bytes if packed).
 struct Matrix {
   const void* data;
   int64_t ld;
 };
 
-// Columns of thread `tid`, by groups of eight (VEC) or a CTA's width apart, and a
-// matrix's row: copied to `region` of shared memory, read from there, or written.
+// A thread's columns, eight together (VEC) or a CTA's width apart, and a matrix's row: copied to `region` of shared memory, read from there, or written.
 template <typename T, int NT, int NV, bool VEC>
 struct Tile {
   static constexpr int kPieces = int(sizeof(T)) / 2;
@@ -150,6 +156,14 @@ struct Tile {
   }
   static __device__ __forceinline__ int column(int g, int i = 0) {
     return VEC ? (g * NT + int(threadIdx.x)) * 8 + i : (g * 8 + i) * NT + int(threadIdx.x);
+  }
+  // Not vectors: the eight columns of group g at p.
+  static __device__ __forceinline__ void singles(const T* p, int cols, int g, Two* v) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = column(g, i) < cols ? to_float(p[column(g, i)]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
   }
   static __device__ __forceinline__ const T* row_of(const Matrix& m, int64_t row) {
     return static_cast<const T*>(m.data) + row * m.ld;
@@ -183,39 +197,53 @@ struct Tile {
       }
     }
   }
-  // Group g of the row in `region`; zeros past the width.
+  // Group g of the row in `region`; zeros past the width (`clear`).
   static __device__ __forceinline__ void get(const char* region, const Matrix& m, int64_t row, int cols, int g, Two* v) {
     if constexpr (VEC) {
       uint4 raw[kPieces];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        raw[i] = column(g) < cols ? *reinterpret_cast<const uint4*>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16)
-                                  : make_uint4(0, 0, 0, 0);
+        raw[i] = *reinterpret_cast<const uint4*>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16);
       Conv<T>::get(raw, v);
     } else {
-      const T* r = reinterpret_cast<const T*>(region + (reinterpret_cast<uintptr_t>(row_of(m, row)) & 15));
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = column(g, i) < cols ? to_float(r[column(g, i)]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+      singles(reinterpret_cast<const T*>(region + (reinterpret_cast<uintptr_t>(row_of(m, row)) & 15)), cols, g, v);
     }
   }
-  // Group g of a vector over the columns, from global memory (L1 after the first row).
-  static __device__ __forceinline__ void vector(const void* base, int cols, int g, Two* v) {
+  // A vector over the columns (a norm's weight, ..), from global memory, L1 after the
+  // first row.  Vector form: loaded before a reduction and converted after it, so that
+  // the loads' latency and the reduction's pass together.  Past the width it holds the
+  // first columns' values, or zeros where they are asked for.
+  struct Vector {
+    uint4 raw[VEC ? NV : 1][kPieces];
+    __device__ __forceinline__ void load(const void* base, int cols, bool zeros = false) {
+      if constexpr (VEC) {
+#pragma unroll
+        for (int g = 0; g < NV; ++g) {
+          const int c = column(g) < cols ? column(g) : 0;
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            raw[g][i] = ld_vector(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + c) + i);
+            if (zeros && column(g) >= cols) raw[g][i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+    }
+    __device__ __forceinline__ void get(const void* base, int cols, int g, Two* v) const {
+      if constexpr (VEC) Conv<T>::get(raw[g], v);
+      else singles(static_cast<const T*>(base), cols, g, v);
+    }
+  };
+  // One group of such a vector, where it is needed.
+  static __device__ __forceinline__ void group(const void* base, int cols, int g, Two* v) {
     const T* p = static_cast<const T*>(base);
     if constexpr (VEC) {
       uint4 raw[kPieces];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        raw[i] = column(g) < cols ? __ldg(reinterpret_cast<const uint4*>(p + column(g)) + i) : make_uint4(0, 0, 0, 0);
+        raw[i] = column(g) < cols ? reinterpret_cast<const uint4*>(p + column(g))[i] : make_uint4(0, 0, 0, 0);
       Conv<T>::get(raw, v);
     } else {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = column(g, i) < cols ? to_float(p[column(g, i)]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
+      singles(p, cols, g, v);
     }
   }
   static __device__ __forceinline__ void store(void* base, int64_t ld, int64_t row, int cols, int g, const Two* v) {
@@ -263,15 +291,9 @@ struct PackedTile {
   static __device__ __forceinline__ void get(const char* region, const Matrix&, int64_t, int cols, int g, Two* v) {
     float f[8];
     if constexpr (VEC) {
-      const int col = C::column(g);
-      uint2 codes = make_uint2(0, 0);
-      unsigned byte = 1;
-      if (col < cols) {
-        codes = *reinterpret_cast<const uint2*>(region + (g * NT + threadIdx.x) * 8);
-        const unsigned four = *reinterpret_cast<const unsigned*>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4);
-        byte = four >> (8 * (col / kPackGroup & 3)) & 0xffu;
-      }
-      decode8(codes, pack_unit(byte), f);
+      const uint2 codes = *reinterpret_cast<const uint2*>(region + (g * NT + threadIdx.x) * 8);
+      const unsigned four = *reinterpret_cast<const unsigned*>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4);
+      decode8(codes, pack_unit(four >> (8 * (C::column(g) / kPackGroup & 3)) & 0xffu), f);
     } else {
       const unsigned char* r = reinterpret_cast<const unsigned char*>(region);
 #pragma unroll
@@ -284,6 +306,16 @@ struct PackedTile {
     for (int i = 0; i < 4; ++i) v[i] = two(f[2 * i], f[2 * i + 1]);
   }
 };
+
+// Vector form: nothing is copied to the places of columns past the width, and what
+// is read from there is zero.
+template <int NT, bool VEC>
+__device__ __forceinline__ void clear(char* ring, int bytes, bool whole) {
+  if (VEC && !whole) {
+    for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();  // other threads' places were cleared here too
+  }
+}
 
 // Walks over a CTA's rows with the next ones on their way: fetch(row, stage) starts
 // the copies of a row, work(row, stage) has them in place.
@@ -359,11 +391,12 @@ __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, floa
 }
 
 template <typename T, int NT, int NV, bool VEC, int STAGES>
-__global__ void __launch_bounds__(NT) join_fwd_kernel(JoinFwd p) {
+__global__ void __launch_bounds__(NT, 512 / NT) join_fwd_kernel(JoinFwd p) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float sh[64];
   using C = Tile<T, NT, NV, VEC>;
   const int bytes = C::bytes(p.cols);
+  clear<NT, VEC>(ring, STAGES * 2 * bytes, p.cols == NT * NV * 8);
   walk<NT, VEC, STAGES>(
       p.rows,
       [&](int64_t row, int stage) {
@@ -374,6 +407,10 @@ __global__ void __launch_bounds__(NT) join_fwd_kernel(JoinFwd p) {
         Two y[NV * 4];
 #pragma unroll
         for (int g = 0; g < NV; ++g) C::get(ring + (2 * stage) * bytes, p.y, row, p.cols, g, y + g * 4);
+        typename C::Vector pw, pb, gate;
+        pw.load(p.pw, p.cols);
+        pb.load(p.pb, p.cols);
+        gate.load(p.gate, p.cols, true);  // columns past the width stay zero in u
         float2 st = row_stats<NT, NV, VEC, C>(y, p, sh);
         if (threadIdx.x == 0) {
           p.stats[row] = st.x;
@@ -384,17 +421,19 @@ __global__ void __launch_bounds__(NT) join_fwd_kernel(JoinFwd p) {
 #pragma unroll
         for (int g = 0; g < NV; ++g) {
           Two w[4], b[4], v[4];
-          C::vector(p.pw, p.cols, g, w);
-          C::vector(p.pb, p.cols, g, b);
+          pw.get(p.pw, p.cols, g, w);
+          pb.get(p.pb, p.cols, g, b);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             y[g * 4 + i] = two_fma(two_mul(two_add(y[g * 4 + i], minus), scale), w[i], b[i]);
-          C::vector(p.gate, p.cols, g, w);
+          gate.get(p.gate, p.cols, g, w);
           C::get(ring + (2 * stage + 1) * bytes, p.x, row, p.cols, g, v);
 #pragma unroll
           for (int i = 0; i < 4; ++i) y[g * 4 + i] = two_fma(w[i], y[g * 4 + i], two_mul(alpha, v[i]));
           C::store(p.u, p.cols, row, p.cols, g, y + g * 4);
         }
+        pw.load(p.w, p.cols);
+        pb.load(p.b, p.cols);
         st = row_stats<NT, NV, VEC, C>(y, p, sh + 32);
         if (threadIdx.x == 0) {
           p.stats[2 * int64_t(p.rows) + row] = st.x;
@@ -404,8 +443,8 @@ __global__ void __launch_bounds__(NT) join_fwd_kernel(JoinFwd p) {
 #pragma unroll
         for (int g = 0; g < NV; ++g) {
           Two w[4], b[4];
-          C::vector(p.w, p.cols, g, w);
-          C::vector(p.b, p.cols, g, b);
+          pw.get(p.w, p.cols, g, w);
+          pb.get(p.b, p.cols, g, b);
 #pragma unroll
           for (int i = 0; i < 4; ++i) b[i] = two_fma(two_mul(two_add(y[g * 4 + i], minus), scale), w[i], b[i]);
           C::store(p.h, p.ld_h, row, p.cols, g, b);
@@ -444,6 +483,45 @@ __global__ void __launch_bounds__(NT, 512 / NT) join_bwd_kernel(JoinBwd p) {
   using C = typename Tiles::C;
   using K = typename Tiles::K;
   const int whole = C::bytes(p.cols), kept = K::bytes(p.cols), bytes = Tiles::bytes(p.cols);
+  clear<NT, VEC>(ring, STAGES * bytes, p.cols == NT * NV * 8);
+  // w and gate * pw in FP32 for this thread's columns: pieces of four, behind the rows.
+  float4* const weights = reinterpret_cast<float4*>(ring + STAGES * bytes);
+  auto keep = [&](int which, int g, const Two* v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 a = both(v[2 * i]), b = both(v[2 * i + 1]);
+      weights[((which * NV + g) * 2 + i) * NT + threadIdx.x] = make_float4(a.x, a.y, b.x, b.y);
+    }
+  };
+  auto weight = [&](int which, int g, Two* v) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 q = weights[((which * NV + g) * 2 + i) * NT + threadIdx.x];
+      v[2 * i] = two(q.x, q.y);
+      v[2 * i + 1] = two(q.z, q.w);
+    }
+  };
+  {
+    typename C::Vector w, pw, gate;
+    w.load(p.w, p.cols, true);
+    if (BRANCH) {
+      pw.load(p.pw, p.cols, true);
+      gate.load(p.gate, p.cols, true);
+    }
+#pragma unroll
+    for (int g = 0; g < NV; ++g) {
+      Two a[4], b[4];
+      w.get(p.w, p.cols, g, a);
+      keep(0, g, a);
+      if (BRANCH) {
+        pw.get(p.pw, p.cols, g, a);
+        gate.get(p.gate, p.cols, g, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = two_mul(a[i], b[i]);
+        keep(1, g, a);
+      }
+    }
+  }
   Two dw[N], db[N], P[BRANCH ? N : 1], Q[BRANCH ? N : 1];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -451,6 +529,10 @@ __global__ void __launch_bounds__(NT, 512 / NT) join_bwd_kernel(JoinBwd p) {
     if (BRANCH) P[i] = Q[i] = 0;
   }
   int turn = 0;  // without a branch: the reductions' buffers alternate
+  // Lanes 0 to 3 of every warp hold the row's four statistics, loaded a row ahead.
+  const int which = threadIdx.x & 3;
+  const float* stats = which == 0 ? p.mean_u : which == 1 || !BRANCH ? p.rstd_u : which == 2 ? p.mean_y : p.rstd_y;
+  float stat = blockIdx.x < p.rows ? stats[blockIdx.x] : 0.f;
   walk<NT, VEC, STAGES>(
       p.rows,
       [&](int64_t row, int stage) {
@@ -462,86 +544,108 @@ __global__ void __launch_bounds__(NT, 512 / NT) join_bwd_kernel(JoinBwd p) {
       },
       [&](int64_t row, int stage) {
         const char* r = ring + stage * bytes;
-        const float mean_u = p.mean_u[row], rstd_u = p.rstd_u[row];
-        float mean_y = 0.f, rstd_y = 0.f;
-        if (BRANCH) {
-          mean_y = p.mean_y[row];
-          rstd_y = p.rstd_y[row];
-        }
-        Two hat[N], a[N], s0 = 0, s1 = 0;
-        {
-          const Two scale = two(rstd_u, rstd_u), minus = two(-mean_u, -mean_u);
+        const float mean_u = __shfl_sync(kAllLanes, stat, 0), rstd_u = __shfl_sync(kAllLanes, stat, 1);
+        const float mean_y = __shfl_sync(kAllLanes, stat, 2), rstd_y = __shfl_sync(kAllLanes, stat, 3);
+        if (row + gridDim.x < p.rows) stat = stats[row + gridDim.x];
+        // hat = (x - mean) rstd, the difference first: a mean far above the spread would
+        // otherwise cost hat the digits that they differ by.
+        const Two scale_u = two(rstd_u, rstd_u), minus_u = two(-mean_u, -mean_u);
+        const Two scale_y = two(rstd_y, rstd_y), minus_y = two(-mean_y, -mean_y);
+        Two s0 = 0, s1 = 0;
+        // Without a branch there are registers to hold a and hat over the reduction; with
+        // one they would spill, and are read and computed again.
+        Two held_a[BRANCH ? 1 : N], held_hat[BRANCH ? 1 : N];
 #pragma unroll
-          for (int g = 0; g < NV; ++g) {
-            Two d[4], w[4];
-            C::get(r, p.dh, row, p.cols, g, d);
-            K::get(r + 2 * whole, p.u, row, p.cols, g, hat + g * 4);
-            C::vector(p.w, p.cols, g, w);
+        for (int g = 0; g < NV; ++g) {
+          Two d[4], hat[4], w[4];
+          C::get(r, p.dh, row, p.cols, g, d);
+          K::get(r + 2 * whole, p.u, row, p.cols, g, hat);
+          weight(0, g, w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = g * 4 + i;
-              hat[k] = two_mul(two_add(hat[k], minus), scale);
-              dw[k] = two_fma(d[i], hat[k], dw[k]);
-              db[k] = two_add(db[k], d[i]);
-              a[k] = two_mul(d[i], w[i]);
-              s0 = two_add(s0, a[k]);
-              s1 = two_fma(a[k], hat[k], s1);
+          for (int i = 0; i < 4; ++i) {
+            hat[i] = two_mul(two_add(hat[i], minus_u), scale_u);
+            dw[g * 4 + i] = two_fma(d[i], hat[i], dw[g * 4 + i]);
+            db[g * 4 + i] = two_add(db[g * 4 + i], d[i]);
+            d[i] = two_mul(d[i], w[i]);
+            s0 = two_add(s0, d[i]);
+            s1 = two_fma(d[i], hat[i], s1);
+            if constexpr (!BRANCH) {
+              held_a[g * 4 + i] = d[i];
+              held_hat[g * 4 + i] = hat[i];
             }
-            if (p.h) {
-              C::vector(p.b, p.cols, g, d);
+          }
+          if (p.h) {
+            Two b[4];
+            C::group(p.b, p.cols, g, b);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) d[i] = two_fma(hat[g * 4 + i], w[i], d[i]);
-              C::store(p.h, p.cols, row, p.cols, g, d);
-            }
+            for (int i = 0; i < 4; ++i) b[i] = two_fma(hat[i], w[i], b[i]);
+            C::store(p.h, p.cols, row, p.cols, g, b);
           }
         }
         float2 m = cta_sum2<NT>(total(s0), total(s1), sh[BRANCH ? 0 : turn]);
         turn ^= 1;
-        {
-          // dt = du + rstd (a - <a> - hat <a hat>)
-          const Two m0 = two(-m.x * p.inverse, -m.x * p.inverse), m1 = two(-m.y * p.inverse, -m.y * p.inverse);
-          const Two rstd = two(rstd_u, rstd_u), alpha = two(p.alpha, p.alpha);
-          const Two scale = two(rstd_y, rstd_y), minus = two(-mean_y, -mean_y);
-          s0 = s1 = 0;
+        // dt = du + rstd (a - <a> - hat <a hat>), as du + a rstd + (h q + r) with q and r of
+        // the row, where h is hat if it was held, or u - mean (rstd is in q then).
+        float q = -m.y * p.inverse * rstd_u, rest = -m.x * p.inverse * rstd_u;
+        if constexpr (BRANCH) q *= rstd_u;
+        Two q2 = two(q, q), rest2 = two(rest, rest);
+        const Two alpha = two(p.alpha, p.alpha);
+        Two c[BRANCH ? N : 1];
+        s0 = s1 = 0;
 #pragma unroll
-          for (int g = 0; g < NV; ++g) {
-            Two d[4] = {0, 0, 0, 0};
-            if (p.du.data) C::get(r + whole, p.du, row, p.cols, g, d);
+        for (int g = 0; g < NV; ++g) {
+          Two d[4], hat[4], w[4], t[4] = {0, 0, 0, 0};
+          if (p.du.data) C::get(r + whole, p.du, row, p.cols, g, t);
+          if constexpr (BRANCH) {
+            C::get(r, p.dh, row, p.cols, g, d);
+            K::get(r + 2 * whole, p.u, row, p.cols, g, hat);
+            weight(0, g, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              d[i] = two_mul(d[i], w[i]);
+              hat[i] = two_add(hat[i], minus_u);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              d[i] = held_a[g * 4 + i];
+              hat[i] = held_hat[g * 4 + i];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            t[i] = two_add(t[i], two_fma(d[i], scale_u, two_fma(hat[i], q2, rest2)));
+            d[i] = two_mul(alpha, t[i]);
+          }
+          C::store(p.dx, p.ld_dx, row, p.cols, g, d);
+          if constexpr (BRANCH) {
+            K::get(r + 2 * whole + kept, p.y, row, p.cols, g, hat);
+            weight(1, g, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int k = g * 4 + i;
-              a[k] = two_fma(two_add(a[k], two_fma(hat[k], m1, m0)), rstd, d[i]);
-              d[i] = two_mul(alpha, a[k]);
-            }
-            C::store(p.dx, p.ld_dx, row, p.cols, g, d);
-            if constexpr (BRANCH) {
-              Two w[4];
-              K::get(r + 2 * whole + kept, p.y, row, p.cols, g, hat + g * 4);
-              C::vector(p.pw, p.cols, g, w);
-              C::vector(p.gate, p.cols, g, d);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int k = g * 4 + i;
-                hat[k] = two_mul(two_add(hat[k], minus), scale);
-                P[k] = two_fma(a[k], hat[k], P[k]);
-                Q[k] = two_add(Q[k], a[k]);
-                a[k] = two_mul(a[k], two_mul(d[i], w[i]));
-                s0 = two_add(s0, a[k]);
-                s1 = two_fma(a[k], hat[k], s1);
-              }
+              hat[i] = two_mul(two_add(hat[i], minus_y), scale_y);
+              P[k] = two_fma(t[i], hat[i], P[k]);
+              Q[k] = two_add(Q[k], t[i]);
+              c[k] = two_mul(t[i], w[i]);
+              s0 = two_add(s0, c[k]);
+              s1 = two_fma(c[k], hat[i], s1);
             }
           }
         }
         if constexpr (BRANCH) {
           m = cta_sum2<NT>(total(s0), total(s1), sh[1]);
-          const Two m0 = two(-m.x * p.inverse, -m.x * p.inverse), m1 = two(-m.y * p.inverse, -m.y * p.inverse);
-          const Two rstd = two(rstd_y, rstd_y);
+          // dy = rstd (c - <c> - yhat <c yhat>) = c rstd + ((y - mean) q + r)
+          q = -m.y * p.inverse * rstd_y * rstd_y;
+          rest = -m.x * p.inverse * rstd_y;
+          q2 = two(q, q), rest2 = two(rest, rest);
 #pragma unroll
           for (int g = 0; g < NV; ++g) {
-            Two d[4];
+            Two hat[4];
+            K::get(r + 2 * whole + kept, p.y, row, p.cols, g, hat);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = two_mul(two_add(a[g * 4 + i], two_fma(hat[g * 4 + i], m1, m0)), rstd);
-            C::store(p.dy, p.ld_dy, row, p.cols, g, d);
+            for (int i = 0; i < 4; ++i) hat[i] = two_fma(c[g * 4 + i], scale_y, two_fma(two_add(hat[i], minus_y), q2, rest2));
+            C::store(p.dy, p.ld_dy, row, p.cols, g, hat);
           }
         }
       });
@@ -626,10 +730,10 @@ int most_ctas(int nt, int ring) {
 
 template <typename T, int NT, int NV, bool VEC>
 int fwd_launch(const JoinFwd& p, cudaStream_t s) {
-  const int smem = kStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
+  const int smem = kFwdStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
   if (smem > kMaxRing) return -1;
-  if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kStages>>(smem)) return r;
-  join_fwd_kernel<T, NT, NV, VEC, kStages><<<unsigned(std::min(p.rows, most_ctas(NT, smem))), NT, smem, s>>>(p);
+  if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kFwdStages>>(smem)) return r;
+  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(NT, smem))), NT, smem, s>>>(p);
   return int(cudaGetLastError());
 }
 template <typename T, bool VEC>
@@ -644,9 +748,9 @@ int fwd_pick(const JoinFwd& p, cudaStream_t s) {
 // The gradient's CTAs: as many as fit, but four rows each where that leaves every SM one.
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
-  // Three rows of the widest FP32 tensors are more than an SM holds.
-  constexpr int kRows = sizeof(T) == 4 && NT == 512 ? 1 : kStages;
-  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols);
+  // Two rows of the widest FP32 tensors are more than an SM holds.
+  constexpr int kRows = sizeof(T) == 4 && NT == 512 ? 1 : kBwdStages;
+  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + (BRANCH ? 2 : 1) * NT * NV * 32;
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
   f.parts = std::min(std::min(p.rows, most_ctas(NT, smem)), std::max(p.rows / 4, 148));

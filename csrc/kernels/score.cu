@@ -8,11 +8,12 @@
 //
 // Forward: a cluster of 1 to 8 CTAs per row, each thread with running (m, s, u)
 // in FP32 over 16-byte vectors; a logit of -inf adds nothing.  The alternatives
-// need no sort of the row: each thread keeps its largest value and the start of
-// the vector that held it.  The k-th largest of these (value, start) pairs
-// bounds the k-th largest logit from below, and only the k threads at or above
-// it can hold one, so a second look at those threads' vectors collects the few
-// candidates, which one warp sorts.  Equal values go to the lowest index.
+// need no sort of the row: the k-th largest of the threads' maxima bounds the k-th
+// largest logit from below, and only the threads that reach it can hold one, so a
+// second look at those threads' vectors collects the few candidates, which one warp
+// sorts.  Equal values go to the lowest index.  Where many values are equal, the
+// threads' maxima are (value, start of the vector that held it), of which no two are
+// the same.
 // Ranks of a vocabulary-parallel group exchange one record a row (m, s, u, z_t
 // and their own alternatives) and merge them in rank order.
 #include <cooperative_groups.h>
@@ -251,10 +252,9 @@ template <> __device__ __forceinline__ float plain_low<__half>() { return -6e4f;
 // difference would be another reference).
 __device__ __forceinline__ float reference(float m) { return __fmul_rn(m, kLog2e); }
 
-template <typename T, bool TOP>
+template <typename T>
 struct Fast {
-  float m = start_low<T>(), best = -INFINITY;
-  unsigned best_at = 0xffffffffu;
+  float m = start_low<T>();
   Two s = 0, u = 0;  // of even and odd elements
 
   __device__ __forceinline__ void raise(float top) {
@@ -272,9 +272,8 @@ struct Fast {
     s = two_add(s, e);
     u = two_fma(e, t, u);
   }
-  // COUNT vectors; `at` is the first one's index and `step` the distance to the next.
   template <int COUNT>
-  __device__ __forceinline__ void add(const uint4* raw, unsigned at, unsigned step) {
+  __device__ __forceinline__ void add(const uint4* raw) {
     constexpr int P = Loaded<T>::kPairs;
     Two z[COUNT * P];
     float top = -INFINITY;
@@ -282,10 +281,6 @@ struct Fast {
     for (int i = 0; i < COUNT; ++i) {
       float t;
       Loaded<T>::read(raw[i], t, z + i * P);
-      if (TOP && t > best) {
-        best = t;
-        best_at = at + i * step;
-      }
       top = max_nan(top, t);
     }
     raise(top);
@@ -294,18 +289,13 @@ struct Fast {
 #pragma unroll
     for (int i = 0; i < COUNT * P; ++i) count(z[i], scale, minus_r);
   }
-  __device__ __forceinline__ void add_one(float v, unsigned at) {
-    if (TOP && v > best) {
-      best = v;
-      best_at = at;
-    }
+  __device__ __forceinline__ void add_one(float v) {
     raise(v);
     const float t = fmaf(fmaxf(v, -kFloor), kLog2e, -reference(m));
     const float e = fast_exp2(t);
     s = two_add(s, two(e, 0.f));
     u = two_fma(two(e, 0.f), two(t, 0.f), u);
   }
-  __device__ __forceinline__ Key key() const { return best_at != 0xffffffffu ? make_key(best, best_at) : 0; }
   // The warp's sums relative to its own maximum, in every lane.
   __device__ __forceinline__ Sums warp_total() const {
     float top = m;
@@ -352,8 +342,91 @@ struct TopShared {
   unsigned active_count, count;
 };
 
-// Descending list of the CTA's 32 best, of which the first k count, in every
-// lane of warp 0 (and in sh.lists[0]).
+__device__ __forceinline__ float exchange(float v, int d, bool larger) {
+  const float o = __shfl_xor_sync(kAllLanes, v, d);
+  return larger ? fmaxf(v, o) : fminf(v, o);
+}
+
+// The warp's sorted list of the candidates that were collected.
+template <int NT>
+__device__ __forceinline__ void sort_candidates(TopShared<NT>& sh, unsigned n) {
+  const int lane = threadIdx.x & 31;
+  Key list = 0;
+  for (unsigned at = 0; at < n; at += 32) {
+    const Key next = sort_warp(at + lane < n ? sh.candidates[at + lane] : 0);
+    list = at ? merge_warp(list, next) : next;
+  }
+  sh.lists[0][lane] = list;
+}
+
+// The CTA's list for a part of ordinary values: by values alone, the index counts only
+// among the candidates.  False (for every thread) where that does not decide: fewer
+// than k threads with ordinary values, or more candidates than there is room for
+// (many equal values); then `block_top` does.
+template <typename T, int NT>
+__device__ __forceinline__ bool fast_top(const Part<T>& part, float own, int k, TopShared<NT>& sh) {
+  constexpr int W = NT / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  float(*const lists)[32] = reinterpret_cast<float(*)[32]>(sh.lists);
+  float v = own;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int d = size >> 1; d; d >>= 1) v = exchange(v, d, ((lane & d) == 0) == (size == 32 || (lane & size) == 0));
+  }
+  lists[warp][lane] = v;
+  if (tid == 0) sh.active_count = sh.count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int half = W / 2; half; half >>= 1) {
+    if (warp < half) {
+      v = fmaxf(v, lists[warp + half][31 - lane]);
+#pragma unroll
+      for (int d = 16; d; d >>= 1) v = exchange(v, d, (lane & d) == 0);
+      lists[warp][lane] = v;
+    }
+    __syncthreads();
+  }
+  const float bound = lists[0][k - 1];
+  if (!(bound > plain_low<T>())) return false;
+  if (own >= bound) sh.active[atomicAdd(&sh.active_count, 1u)] = tid;
+  __syncthreads();
+  auto take = [&](float value, unsigned index) {
+    if (value >= bound) {
+      const unsigned at = atomicAdd(&sh.count, 1u);
+      if (at < kCandidates) sh.candidates[at] = make_key(value, index);
+    }
+  };
+  // A warp for each active thread: its vectors are NT apart.
+  for (unsigned a = warp; a < sh.active_count; a += W) {
+    for (unsigned j = sh.active[a] + lane * NT; j < part.vectors; j += 32 * NT) {
+      const unsigned at = part.vector_at(j);
+      const uint4 raw = *reinterpret_cast<const uint4*>(part.x + at);
+      Vec<T> vec;
+      vec.raw = raw;
+      float z[Vec<T>::kN];
+      vec.get(z);
+      float top = z[0];
+#pragma unroll
+      for (int e = 1; e < Vec<T>::kN; ++e) top = fmaxf(top, z[e]);
+      if (top < bound) continue;  // most vectors hold none
+#pragma unroll
+      for (int e = 0; e < Vec<T>::kN; ++e) take(z[e], part.lo + at + e);
+    }
+  }
+  for (unsigned c = tid; c < part.head + part.tail; c += NT) {
+    const unsigned at = c < part.head ? c : part.vector_at(part.vectors) + (c - part.head);
+    take(to_float(part.x[at]), part.lo + at);
+  }
+  __syncthreads();
+  const unsigned n = sh.count;
+  if (n > kCandidates) return false;
+  if (warp == 0) sort_candidates(sh, n);
+  return true;
+}
+
+// The same for any values, equal ones and NaN.  Descending list of the CTA's 32 best,
+// of which the first k count, in sh.lists[0].
 template <typename T, int NT>
 __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, TopShared<NT>& sh) {
   constexpr int W = NT / 32;
@@ -389,6 +462,10 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
         float v[Vec<T>::kN];
         vec.load(part.x + at);
         vec.get(v);
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < Vec<T>::kN; ++e) top = max_nan(top, v[e]);
+        if (make_key(top, part.lo + at) < bound) continue;  // most vectors hold none
 #pragma unroll
         for (int e = 0; e < Vec<T>::kN; ++e)
           if (make_key(v[e], part.lo + at) >= bound) take(make_key(v[e], part.lo + at + e));
@@ -407,14 +484,7 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
   __syncthreads();
   const unsigned n = sh.count;
   if (n <= kCandidates) {
-    if (warp == 0) {
-      list = 0;
-      for (unsigned at = 0; at < n; at += 32) {
-        const Key next = sort_warp(at + lane < n ? sh.candidates[at + lane] : 0);
-        list = at ? merge_warp(list, next) : next;
-      }
-      sh.lists[0][lane] = list;
-    }
+    if (warp == 0) sort_candidates(sh, n);
   } else {
     // Many candidates in few threads' vectors: the k largest one after another.
     Key below = ~Key(0);
@@ -462,35 +532,37 @@ __global__ void __launch_bounds__(NT) score_kernel(const T* logits, int64_t ld, 
 
   // Sums of the CTA's part: by the fast form, or by the definitions where the
   // largest value says that the fast one does not hold.
-  Key key = 0;
+  float own;  // the thread's largest value
   {
-    Fast<T, TOP> run;
-    if (unsigned(tid) < part.head) run.add_one(to_float(part.x[tid]), part.lo + tid);
+    Fast<T> run;
+    if (unsigned(tid) < part.head) run.add_one(to_float(part.x[tid]));
     const uint4* vectors = reinterpret_cast<const uint4*>(part.x + part.head);
     unsigned j = tid;
     for (; j + (kUnroll - 1) * NT < part.vectors; j += kUnroll * NT) {
       uint4 raw[kUnroll];
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) raw[i] = vectors[j + i * NT];
-      run.template add<kUnroll>(raw, part.lo + part.vector_at(j), NT * kN);
+      run.template add<kUnroll>(raw);
     }
     for (; j < part.vectors; j += NT) {
       const uint4 raw = vectors[j];
-      run.template add<1>(&raw, part.lo + part.vector_at(j), 0);
+      run.template add<1>(&raw);
     }
     if (unsigned(tid) < part.tail) {
-      const unsigned i = part.vector_at(part.vectors) + tid;
-      run.add_one(to_float(part.x[i]), part.lo + i);
+      run.add_one(to_float(part.x[part.vector_at(part.vectors) + tid]));
     }
     const Sums a = run.warp_total();
-    if (TOP) key = run.key();
+    own = run.m;
     if (lane == 0) warp_sums[warp] = a;
   }
   __syncthreads();
   float top = warp_sums[0].m;
 #pragma unroll
   for (int w = 1; w < W; ++w) top = max_nan(top, warp_sums[w].m);
-  const bool plain = top > plain_low<T>() && top < kPlain;
+  bool plain = top > plain_low<T>() && top < kPlain;
+  if constexpr (TOP) {
+    if (plain) plain = fast_top(part, own, o.k, sh);
+  }
   if (plain) {
     if (tid == 0) {
       Sums a{top, 0.f, 0.f};
@@ -539,9 +611,8 @@ __global__ void __launch_bounds__(NT) score_kernel(const T* logits, int64_t ld, 
       for (int w = 1; w < W; ++w) a = join(a, warp_sums[w]);
       block_sums = a;
     }
-    if (TOP) key = run.key();
+    if constexpr (TOP) block_top(part, run.key(), o.k, sh);  // synchronises
   }
-  if constexpr (TOP) block_top(part, key, o.k, sh);  // synchronises
   if (C > 1) cluster.sync();
   else __syncthreads();
   if (rank == 0 && warp == 0) {
@@ -682,7 +753,7 @@ int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* 
                                 start, vocab_total, chunk, o));
 }
 // Threads of a row's CTA, and CTAs an SM takes at once.
-constexpr int kRowThreads = 128, kRowCtas = 8;
+constexpr int kRowThreads = 256, kRowCtas = 5;
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
