@@ -72,14 +72,24 @@ __device__ __forceinline__ float2 cta_sum2(float a, float b, float2* sh) {
   } else {
     if ((threadIdx.x & 15) == 0) reinterpret_cast<float*>(sh)[threadIdx.x >> 4] = v;
     __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
+    if constexpr (NT <= 128) {
+      float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
-      const float4 q = reinterpret_cast<const float4*>(sh)[w];
-      s.x += q.x + q.z;
-      s.y += q.y + q.w;
+      for (int w = 0; w < NT / 64; ++w) {
+        const float4 q = reinterpret_cast<const float4*>(sh)[w];
+        s.x += q.x + q.z;
+        s.y += q.y + q.w;
+      }
+      return s;
+    } else {  // a lane for each warp's pair
+      float2 s = sh[threadIdx.x & (NT / 32 - 1)];
+#pragma unroll
+      for (int d = NT / 64; d; d >>= 1) {
+        s.x += __shfl_xor_sync(kAllLanes, s.x, d);
+        s.y += __shfl_xor_sync(kAllLanes, s.y, d);
+      }
+      return s;
     }
-    return s;
   }
 }
 __device__ __forceinline__ float total(Two v) {
@@ -464,6 +474,10 @@ struct JoinBwd {
   float alpha, inverse;
 };
 
+// Threads of the gradient on an SM: 64 registers each for eight columns a thread, 128
+// for sixteen.
+__host__ __device__ constexpr int bwd_threads(int) { return 512; }
+
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 struct BwdTiles {
   using C = Tile<T, NT, NV, VEC>;
@@ -475,7 +489,7 @@ struct BwdTiles {
 // values that the first decides.  The column sums stay in registers: 64 of them for
 // sixteen columns a thread, which is what limits an SM to 512 threads.
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
-__global__ void __launch_bounds__(NT, 512 / NT) join_bwd_kernel(JoinBwd p) {
+__global__ void __launch_bounds__(NT, bwd_threads(NV) / NT) join_bwd_kernel(JoinBwd p) {
   constexpr int N = NV * 4;
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float2 sh[2][16];
@@ -721,10 +735,9 @@ int opt_in(int smem) {
   if (e == cudaSuccess) opted.fetch_or(bit, std::memory_order_relaxed);
   return int(e);
 }
-// CTAs of 512 / NT or what the rings leave room for, on every SM.
-int most_ctas(int nt, int ring) {
+// CTAs that an SM takes by threads or by what their rings leave room for, on every SM.
+int most_ctas(int by_threads, int ring) {
   const int fit = kMaxRing / (ring > 0 ? ring : 1);
-  const int by_threads = 512 / nt;
   return 148 * (fit < by_threads ? (fit < 1 ? 1 : fit) : by_threads);
 }
 
@@ -733,7 +746,7 @@ int fwd_launch(const JoinFwd& p, cudaStream_t s) {
   const int smem = kFwdStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kFwdStages>>(smem)) return r;
-  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(NT, smem))), NT, smem, s>>>(p);
+  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(512 / NT, smem))), NT, smem, s>>>(p);
   return int(cudaGetLastError());
 }
 template <typename T, bool VEC>
@@ -753,7 +766,7 @@ int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + (BRANCH ? 2 : 1) * NT * NV * 32;
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
-  f.parts = std::min(std::min(p.rows, most_ctas(NT, smem)), std::max(p.rows / 4, 148));
+  f.parts = std::min(std::min(p.rows, most_ctas(bwd_threads(NV) / NT, smem)), std::max(p.rows / 4, 148));
   join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
   if (const int r = int(cudaGetLastError())) return r;
   join_finish_kernel<T, BRANCH><<<unsigned((p.cols + 31) / 32), 1024, 0, s>>>(f);
@@ -772,8 +785,8 @@ int bwd_pick(const JoinBwd& p, const JoinFinish& f, cudaStream_t s) {
 int64_t join_max_cols() { return kJoinMaxCols; }
 int join_bwd_parts(int64_t rows, int64_t cols) {
   // The most that any form launches at this width (threads alone).
-  const int nt = cols <= 256 ? 32 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
-  return int(std::min<int64_t>(rows, 148 * (512 / nt)));
+  const int per_sm = cols <= 256 ? 32 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;
+  return int(std::min<int64_t>(rows, 148 * per_sm));
 }
 
 int join_fwd(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int type, const void* pw, const void* pb,

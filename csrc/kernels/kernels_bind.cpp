@@ -430,8 +430,9 @@ Tensors token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int6
   at::Tensor out = at::empty({rows * (5 + top_k)}, logits.options().dtype(at::kFloat));
   at::Tensor ids = at::empty({rows, top_k}, logits.options().dtype(at::kLong));
   if (rows) score_fwd(logits, targets.contiguous(), 0, logits.size(1), top_k, out, ids, c10::nullopt);
-  return {out.narrow(0, 0, rows), out.narrow(0, rows, rows), out.narrow(0, 5 * rows, rows * top_k).view({rows, top_k}),
-          ids, out.narrow(0, 2 * rows, 3 * rows).view({3, rows})};
+  return {out.as_strided({rows}, {1}, 0), out.as_strided({rows}, {1}, rows),
+          out.as_strided({rows, top_k}, {std::max<int64_t>(top_k, 1), 1}, 5 * rows), ids,
+          out.as_strided({3, rows}, {std::max<int64_t>(rows, 1), 1}, 2 * rows)};
 }
 at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& targets, int64_t start,
                                    int64_t vocab_total, const at::Tensor& state, const at::Tensor& dlogprob,

@@ -33,6 +33,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;  // of the merge and the g
 constexpr int kMaxTop = 32;       // alternatives a row: one sorted list per warp
 constexpr int kCandidates = 1024;  // 8 KB; more than that takes the selection by rounds
 constexpr int kUnroll = 4;
+constexpr int kRowThreads = 256, kRowCtas = 6;  // threads of a row's CTA, CTAs an SM takes at once
 constexpr float kLog2e = 1.44269504088896340736f;
 // e^d with d below this is zero in FP32; it also keeps 0 * (-inf) out of u.
 constexpr float kLowest = -200.f;
@@ -514,7 +515,7 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
 
 // grid = rows * C CTAs in clusters of C; the cluster's CTAs take `chunk` columns each.
 template <typename T, bool TOP, int NT>
-__global__ void __launch_bounds__(NT) score_kernel(const T* logits, int64_t ld, unsigned vocab,
+__global__ void __launch_bounds__(NT, kRowCtas) score_kernel(const T* logits, int64_t ld, unsigned vocab,
                                                          const int64_t* targets, int64_t start,
                                                          int64_t vocab_total, unsigned chunk, Out o) {
   constexpr int W = NT / 32;
@@ -681,8 +682,10 @@ __global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, in
                                                              const float* dlogprob, const float* dentropy, T* out,
                                                              int64_t ld_out, unsigned blocks) {
   constexpr int kN = Vec<T>::kN;
-  const int row = blockIdx.x / blocks;
-  const unsigned block = blockIdx.x - unsigned(row) * blocks;
+  // The last rows first: they are what the forward pass, just before this one in most
+  // programs, left in L2.
+  const unsigned place = blockIdx.x / blocks, block = blockIdx.x - place * blocks;
+  const int row = rows - 1 - int(place);
   const float m = state[row], ln_s = state[rows + row], H = state[2 * int64_t(rows) + row];
   const int64_t target = targets[row];
   float a = target >= 0 ? dlogprob[row] : 0.f;
@@ -752,8 +755,6 @@ int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* 
   return int(cudaLaunchKernelEx(&config, score_kernel<T, TOP, NT>, static_cast<const T*>(logits), ld, vocab, targets,
                                 start, vocab_total, chunk, o));
 }
-// Threads of a row's CTA, and CTAs an SM takes at once.
-constexpr int kRowThreads = 256, kRowCtas = 5;
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
