@@ -498,21 +498,20 @@ __global__ void __launch_bounds__(NT, bwd_threads(NV) / NT) join_bwd_kernel(Join
   using K = typename Tiles::K;
   const int whole = C::bytes(p.cols), kept = K::bytes(p.cols), bytes = Tiles::bytes(p.cols);
   clear<NT, VEC>(ring, STAGES * bytes, p.cols == NT * NV * 8);
-  // w and gate * pw in FP32 for this thread's columns: pieces of four, behind the rows.
-  float4* const weights = reinterpret_cast<float4*>(ring + STAGES * bytes);
-  auto keep = [&](int which, int g, const Two* v) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 a = both(v[2 * i]), b = both(v[2 * i + 1]);
-      weights[((which * NV + g) * 2 + i) * NT + threadIdx.x] = make_float4(a.x, a.y, b.x, b.y);
-    }
-  };
+  // For this thread's columns, behind the rows: w as stored, and gate * pw in FP32.
+  uint4* const weights = reinterpret_cast<uint4*>(ring + STAGES * bytes);
+  constexpr int kW = NV * C::kPieces * NT;  // pieces of w
   auto weight = [&](int which, int g, Two* v) {
+    if (which == 0) {
+      uint4 raw[C::kPieces];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float4 q = weights[((which * NV + g) * 2 + i) * NT + threadIdx.x];
-      v[2 * i] = two(q.x, q.y);
-      v[2 * i + 1] = two(q.z, q.w);
+      for (int i = 0; i < C::kPieces; ++i) raw[i] = weights[(g * C::kPieces + i) * NT + threadIdx.x];
+      Conv<T>::get(raw, v);
+    } else {
+      uint4 raw[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) raw[i] = weights[kW + (g * 2 + i) * NT + threadIdx.x];
+      Conv<float>::get(raw, v);
     }
   };
   {
@@ -525,14 +524,19 @@ __global__ void __launch_bounds__(NT, bwd_threads(NV) / NT) join_bwd_kernel(Join
 #pragma unroll
     for (int g = 0; g < NV; ++g) {
       Two a[4], b[4];
+      uint4 raw[2];
       w.get(p.w, p.cols, g, a);
-      keep(0, g, a);
+      Conv<T>::put(a, raw);  // exact: the values came from this type
+#pragma unroll
+      for (int i = 0; i < C::kPieces; ++i) weights[(g * C::kPieces + i) * NT + threadIdx.x] = raw[i];
       if (BRANCH) {
         pw.get(p.pw, p.cols, g, a);
         gate.get(p.gate, p.cols, g, b);
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = two_mul(a[i], b[i]);
-        keep(1, g, a);
+        Conv<float>::put(a, raw);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) weights[kW + (g * 2 + i) * NT + threadIdx.x] = raw[i];
       }
     }
   }
@@ -763,7 +767,7 @@ template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   // Two rows of the widest FP32 tensors are more than an SM holds.
   constexpr int kRows = sizeof(T) == 4 && NT == 512 ? 1 : kBwdStages;
-  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + (BRANCH ? 2 : 1) * NT * NV * 32;
+  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
   f.parts = std::min(std::min(p.rows, most_ctas(bwd_threads(NV) / NT, smem)), std::max(p.rows / 4, 148));

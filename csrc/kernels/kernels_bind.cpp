@@ -349,13 +349,15 @@ int64_t join_bwd_workspace(int64_t rows, int64_t cols, bool branch) {
 // Gradients of the joint, or of LayerNorm alone where `y` is absent.  `u` and `y` are
 // both packed (bytes) or both of dh's type.  grads: dpre_weight, dpre_bias and, with a
 // branch, dpost_weight, dpost_bias, dgate, [2 or 5, cols].
-void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const at::Tensor& u,
-              const c10::optional<at::Tensor>& y, const at::Tensor& mean_u, const at::Tensor& rstd_u,
-              const c10::optional<at::Tensor>& mean_y, const c10::optional<at::Tensor>& rstd_y,
-              const c10::optional<at::Tensor>& pw, const c10::optional<at::Tensor>& pb,
-              const c10::optional<at::Tensor>& gate, const at::Tensor& w, const c10::optional<at::Tensor>& b,
-              at::Tensor& dx, const c10::optional<at::Tensor>& dy, const c10::optional<at::Tensor>& h,
-              at::Tensor& grads, at::Tensor& workspace, double alpha) {
+struct RowStats {  // FP32 [rows] each; *_y without a branch: null
+  const float *mean_u, *rstd_u, *mean_y, *rstd_y;
+};
+void run_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const at::Tensor& u,
+                  const c10::optional<at::Tensor>& y, const RowStats& stats, const c10::optional<at::Tensor>& pw,
+                  const c10::optional<at::Tensor>& pb, const c10::optional<at::Tensor>& gate, const at::Tensor& w,
+                  const c10::optional<at::Tensor>& b, const at::Tensor& dx, const c10::optional<at::Tensor>& dy,
+                  const c10::optional<at::Tensor>& h, const at::Tensor& grads, const at::Tensor& workspace,
+                  double alpha) {
   k::JoinBwdCall c = {};
   c.type = type_code(dh, false, "dh");
   const int64_t rows = dh.size(0), cols = dh.size(1);
@@ -369,12 +371,11 @@ void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const a
     else need_rows(t, dh, rows, cols, name);
   };
   kept(u, "x_out");
-  need_floats(mean_u, dh, rows, "mean"); need_floats(rstd_u, dh, rows, "rstd");
   need_vector(w, dh, cols, "pre_weight");
   c.dh = dh.data_ptr(); c.ld_dh = dh.stride(0);
   c.dx = dx.data_ptr(); c.ld_dx = dx.stride(0);
   c.u = u.data_ptr(); c.ld_u = u.stride(0);
-  c.mean_u = mean_u.data_ptr<float>(); c.rstd_u = rstd_u.data_ptr<float>();
+  c.mean_u = stats.mean_u; c.rstd_u = stats.rstd_u;
   c.w = w.data_ptr();
   if (du) {
     need_rows(*du, dh, rows, cols, "dx_out");
@@ -394,15 +395,14 @@ void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const a
   char* gp = static_cast<char*>(grads.data_ptr());
   c.dw = gp; c.db = gp + step;
   if (branch) {
-    TORCH_CHECK(dy && pw && pb && gate && mean_y && rstd_y, "the branch's tensors go together");
+    TORCH_CHECK(dy && pw && pb && gate && stats.mean_y && stats.rstd_y, "the branch's tensors go together");
     kept(*y, "y");
     need_rows(*dy, dh, rows, cols, "dy");
-    need_floats(*mean_y, dh, rows, "mean_y"); need_floats(*rstd_y, dh, rows, "rstd_y");
     need_vector(*pw, dh, cols, "post_weight"); need_vector(*pb, dh, cols, "post_bias");
     need_vector(*gate, dh, cols, "gate");
     c.y = y->data_ptr(); c.ld_y = y->stride(0);
     c.dy = dy->data_ptr(); c.ld_dy = dy->stride(0);
-    c.mean_y = mean_y->data_ptr<float>(); c.rstd_y = rstd_y->data_ptr<float>();
+    c.mean_y = stats.mean_y; c.rstd_y = stats.rstd_y;
     c.pw = pw->data_ptr(); c.pb = pb->data_ptr(); c.gate = gate->data_ptr();
     c.dpw = gp + 2 * step; c.dpb = gp + 3 * step; c.dgate = gp + 4 * step;
   }
@@ -410,6 +410,22 @@ void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const a
   c.workspace = workspace.data_ptr<float>();
   const c10::cuda::CUDAGuard g(dh.device());
   ok(k::join_bwd(c, cur()), branch ? "block_join_bwd" : "layer_norm_bwd_packed");
+}
+void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const at::Tensor& u,
+              const c10::optional<at::Tensor>& y, const at::Tensor& mean_u, const at::Tensor& rstd_u,
+              const c10::optional<at::Tensor>& mean_y, const c10::optional<at::Tensor>& rstd_y,
+              const c10::optional<at::Tensor>& pw, const c10::optional<at::Tensor>& pb,
+              const c10::optional<at::Tensor>& gate, const at::Tensor& w, const c10::optional<at::Tensor>& b,
+              at::Tensor& dx, const c10::optional<at::Tensor>& dy, const c10::optional<at::Tensor>& h,
+              at::Tensor& grads, at::Tensor& workspace, double alpha) {
+  const int64_t rows = dh.size(0);
+  need_floats(mean_u, dh, rows, "mean"); need_floats(rstd_u, dh, rows, "rstd");
+  RowStats stats{mean_u.data_ptr<float>(), rstd_u.data_ptr<float>(), nullptr, nullptr};
+  if (mean_y && rstd_y) {
+    need_floats(*mean_y, dh, rows, "mean_y"); need_floats(*rstd_y, dh, rows, "rstd_y");
+    stats.mean_y = mean_y->data_ptr<float>(); stats.rstd_y = rstd_y->data_ptr<float>();
+  }
+  run_join_bwd(dh, du, u, y, stats, pw, pb, gate, w, b, dx, dy, h, grads, workspace, alpha);
 }
 
 // The operators' public forms: outputs are allocated here, so that a call costs one
@@ -496,18 +512,22 @@ Tensors block_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du
                        const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& workspace, double alpha) {
   need_matrix(dh, "dh");
   need_own_rows(out, "out");
-  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == 4 && stats.size(1) == dh.size(0) && stats.is_contiguous(),
-              "stats must be contiguous [4, rows]");
+  const int64_t rows = dh.size(0);
+  need_like(stats, dh, at::kFloat, "stats");
+  TORCH_CHECK(stats.dim() == 2 && stats.size(0) == 4 && stats.size(1) == rows, "stats must be [4, rows]");
   TORCH_CHECK(u.scalar_type() == y.scalar_type(), "x_out and y are kept in the same form");
   Spare spare(dh, true, workspace);
   at::Tensor dx = rows_like(dh);
   c10::optional<at::Tensor> dy = out ? *out : rows_like(dh), h;
   if (b) h = rows_like(dh);
-  if (dh.size(0))
-    join_bwd(dh, du, u, y, stats.select(0, 2), stats.select(0, 3), stats.select(0, 0), stats.select(0, 1), pw, pb,
-             gate, w, b, dx, dy, h, spare.grads, spare.workspace, alpha);
-  const at::Tensor& g = spare.grads;
-  return {dx, dy, g.select(0, 2), g.select(0, 3), g.select(0, 4), g.select(0, 0), g.select(0, 1), h};
+  if (rows) {
+    const float* s = stats.data_ptr<float>();
+    run_join_bwd(dh, du, u, y, RowStats{s + 2 * rows, s + 3 * rows, s, s + rows}, pw, pb, gate, w, b, dx, dy, h,
+                 spare.grads, spare.workspace, alpha);
+  }
+  const int64_t cols = dh.size(1);
+  auto grad = [&](int i) { return spare.grads.as_strided({cols}, {1}, i * cols); };
+  return {dx, dy, grad(2), grad(3), grad(4), grad(0), grad(1), h};
 }
 // (dx, dweight, dbias, y)
 Tensors layer_norm_bwd_packed(const at::Tensor& dy, const c10::optional<at::Tensor>& dres, const at::Tensor& x,
@@ -518,13 +538,14 @@ Tensors layer_norm_bwd_packed(const at::Tensor& dy, const c10::optional<at::Tens
   need_own_rows(out, "out");
   TORCH_CHECK(mean.dim() == 1 && rstd.dim() == 1 && mean.numel() == dy.size(0) && rstd.numel() == dy.size(0),
               "mean and rstd must hold one value a row");
+  need_like(mean, dy, at::kFloat, "mean"); need_like(rstd, dy, at::kFloat, "rstd");
   Spare spare(dy, false, workspace);
   at::Tensor dx = out ? *out : rows_like(dy);
   c10::optional<at::Tensor> y, none;
   if (b) y = rows_like(dy);
   if (dy.size(0))
-    join_bwd(dy, dres, x, none, mean, rstd, none, none, none, none, none, w, b, dx, none, y, spare.grads,
-             spare.workspace, 1.0);
+    run_join_bwd(dy, dres, x, none, RowStats{mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr}, none,
+                 none, none, w, b, dx, none, y, spare.grads, spare.workspace, 1.0);
   return {dx, spare.grads.select(0, 0), spare.grads.select(0, 1), y};
 }
 }  // namespace
