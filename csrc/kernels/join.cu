@@ -19,8 +19,8 @@
 // the CTAs in order, without atomics.
 //
 // Both directions are persistent: a CTA takes the rows row, row + grid, .. and has
-// the next two on their way into shared memory (cp.async) while it works on one, so
-// loads are in flight all the time and no register holds them.
+// the next ones (two forward, one backward) on their way into shared memory (cp.async)
+// while it works on one, so loads are in flight all the time and no register holds them.
 //   Vector form (width a multiple of 8, rows on 16-byte boundaries): a thread has
 // eight consecutive columns at a time and copies what it will read itself, so it
 // waits for its own copies alone.
@@ -39,6 +39,7 @@ namespace kernels {
 namespace {
 constexpr int kMaxRing = 200 * 1024;  // of an SM's 227 KB, for all CTAs on it
 constexpr int kFwdStages = 3, kBwdStages = 2;
+constexpr int kSmThreads = 512;  // of all CTAs on an SM, at 128 registers each
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -401,7 +402,7 @@ __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, floa
 }
 
 template <typename T, int NT, int NV, bool VEC, int STAGES>
-__global__ void __launch_bounds__(NT, 512 / NT) join_fwd_kernel(JoinFwd p) {
+__global__ void __launch_bounds__(NT, kSmThreads / NT) join_fwd_kernel(JoinFwd p) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float sh[64];
   using C = Tile<T, NT, NV, VEC>;
@@ -474,10 +475,6 @@ struct JoinBwd {
   float alpha, inverse;
 };
 
-// Threads of the gradient on an SM: 64 registers each for eight columns a thread, 128
-// for sixteen.
-__host__ __device__ constexpr int bwd_threads(int) { return 512; }
-
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 struct BwdTiles {
   using C = Tile<T, NT, NV, VEC>;
@@ -489,7 +486,7 @@ struct BwdTiles {
 // values that the first decides.  The column sums stay in registers: 64 of them for
 // sixteen columns a thread, which is what limits an SM to 512 threads.
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
-__global__ void __launch_bounds__(NT, bwd_threads(NV) / NT) join_bwd_kernel(JoinBwd p) {
+__global__ void __launch_bounds__(NT, kSmThreads / NT) join_bwd_kernel(JoinBwd p) {
   constexpr int N = NV * 4;
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float2 sh[2][16];
@@ -750,7 +747,7 @@ int fwd_launch(const JoinFwd& p, cudaStream_t s) {
   const int smem = kFwdStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kFwdStages>>(smem)) return r;
-  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(512 / NT, smem))), NT, smem, s>>>(p);
+  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(kSmThreads / NT, smem))), NT, smem, s>>>(p);
   return int(cudaGetLastError());
 }
 template <typename T, bool VEC>
@@ -770,7 +767,7 @@ int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
-  f.parts = std::min(std::min(p.rows, most_ctas(bwd_threads(NV) / NT, smem)), std::max(p.rows / 4, 148));
+  f.parts = std::min(std::min(p.rows, most_ctas(kSmThreads / NT, smem)), std::max(p.rows / 4, 148));
   join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
   if (const int r = int(cudaGetLastError())) return r;
   join_finish_kernel<T, BRANCH><<<unsigned((p.cols + 31) / 32), 1024, 0, s>>>(f);
@@ -789,8 +786,8 @@ int bwd_pick(const JoinBwd& p, const JoinFinish& f, cudaStream_t s) {
 int64_t join_max_cols() { return kJoinMaxCols; }
 int join_bwd_parts(int64_t rows, int64_t cols) {
   // The most that any form launches at this width (threads alone).
-  const int per_sm = cols <= 256 ? 32 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;
-  return int(std::min<int64_t>(rows, 148 * per_sm));
+  const int nt = cols <= 256 ? 32 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  return int(std::min<int64_t>(rows, 148 * (kSmThreads / nt)));
 }
 
 int join_fwd(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int type, const void* pw, const void* pb,

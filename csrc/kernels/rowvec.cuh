@@ -25,11 +25,7 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <typename T>
 struct Eight {
   uint4 raw[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < int(sizeof(T) / 2); ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  // Rows that are read once: kept out of L1 so that weights stay there.
+  // Values that are read once pass by L1.
   __device__ __forceinline__ void load_once(const T* p) {
 #pragma unroll
     for (int i = 0; i < int(sizeof(T) / 2); ++i) {
@@ -38,19 +34,10 @@ struct Eight {
                    : "l"(reinterpret_cast<const uint4*>(p) + i));
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-    for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
-  }
   __device__ __forceinline__ void get(float* v) const {
     const T* h = reinterpret_cast<const T*>(raw);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_float(h[i]);
-  }
-  __device__ __forceinline__ void set(const float* v) {
-    T* h = reinterpret_cast<T*>(raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_float<T>(v[i]);
   }
 };
 

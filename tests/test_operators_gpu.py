@@ -458,3 +458,43 @@ def test_refusals_of_the_native_entries():
         lib().join_bwd(x, None, p.data, None, x.new_zeros(4, dtype=FP32), x.new_zeros(4, dtype=FP32), None, None, None,
                        None, None, x[0], None, torch.empty_like(x), None, None, x.new_zeros(2, 64),
                        torch.empty(3, device="cuda"), 1.0)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 50304), (3, 20001), (900, 4001)])
+def test_scores_in_a_captured_graph(rows, V):
+    """Rows split over a cluster, and rows of their own, replayed on new logits."""
+    _, loss, _ = ops()
+    z = randn(16, rows, V, std=3.0)
+    t = torch.randint(0, V, (rows,), generator=gen(17), device="cuda")
+    a = randn(18, rows, to=FP32)
+    loss.token_logprobs(z, t, top_k=20)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, state = loss.token_logprobs(z, t, top_k=20)
+        g = loss.token_logprobs_backward(z, t, state, a)
+    for seed in (19, 20):
+        z.copy_(randn(seed, rows, V, std=3.0))
+        graph.replay()
+        want, ws = loss.token_logprobs(z, t, top_k=20)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        assert torch.equal(g, loss.token_logprobs_backward(z, t, ws, a))
+        ref.check_scores(got, z, t, 20)
+
+
+def test_outputs_may_take_the_place_of_inputs():
+    """dy over dh, and LayerNorm's dx over the gradient it joins: a row is written after it is read."""
+    actpack, _, norm = ops()
+    for rows, H in ((700, 512), (333, 1001)):
+        j = joint(20, rows, H, BF16)
+        x_out, h, stats = norm.block_join_fwd(*j.values(), 1e-5)
+        dh, du = randn(21, rows, H), randn(22, rows, H)
+        args = (x_out, j["y"], stats, j["pw"], j["pb"], j["gate"], j["w"])
+        want = norm.block_join_bwd(dh, du, *args)
+        work = dh.clone()
+        got = norm.block_join_bwd(work, du, *args, out=work)
+        assert all(torch.equal(p, q) for p, q in zip(got[:7], want[:7]))
+        p = actpack.pack(x_out)
+        want = norm.layer_norm_bwd_packed(dh, p, j["w"], stats[2], stats[3], dres=du)
+        work = du.clone()
+        got = norm.layer_norm_bwd_packed(dh, p, j["w"], stats[2], stats[3], dres=work, out=work)
+        assert all(torch.equal(p, q) for p, q in zip(got[:3], want[:3]))
