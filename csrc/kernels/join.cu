@@ -684,41 +684,52 @@ struct JoinFinish {
   int parts, cols;
 };
 
-// 32 columns a CTA; each of its 32 warps adds every 32nd partial sum, in order.
-template <typename T, bool BRANCH>
+// The CTA's 32 warps add every 32nd partial sum, in order, then one warp adds those.
+// WIDE: a lane has all K sums of one column; otherwise one sum, and the CTA 32 / K
+// columns (whole sectors of 32 bytes), since narrow widths have few CTAs here and many
+// partial sums: 11 us against 14 at 8192 x 256, but 10 against 7 at 8192 x 4096.
+template <typename T, bool BRANCH, bool WIDE>
 __global__ void __launch_bounds__(1024) join_finish_kernel(JoinFinish p) {
-  constexpr int K = BRANCH ? 4 : 2;
-  __shared__ float sh[K][32][33];
+  constexpr int K = BRANCH ? 4 : 2, kCols = WIDE ? 32 : 32 / K, kEach = WIDE ? K : 1;
+  __shared__ float sh[kEach][32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + lane;
-  float s[K] = {};
-  if (col < p.cols) {
+  const int col = blockIdx.x * kCols + lane % kCols;
+  const bool has = col < p.cols;
+  float s[kEach] = {};
+  if (has) {
+    const float* from = p.sums + int64_t(lane / kCols) * p.cols + col;
 #pragma unroll 4
     for (int q = part; q < p.parts; q += 32) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) s[k] += p.sums[(int64_t(q) * K + k) * p.cols + col];
+      for (int k = 0; k < kEach; ++k) s[k] += from[(int64_t(q) * K + k) * p.cols];
     }
   }
 #pragma unroll
-  for (int k = 0; k < K; ++k) sh[k][part][lane] = s[k];
+  for (int k = 0; k < kEach; ++k) sh[k][part][lane] = s[k];
   __syncthreads();
-  // Warp k sums the k-th column sum of the 32 columns; warp 0 writes.
-  if (part < K) {
-    float v = 0.f;
+  if (part >= kEach) return;
+  float v = 0.f;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) v += sh[part][q][lane];
-    sh[part][0][lane] = v;
-  }
-  __syncthreads();
-  if (part || col >= p.cols) return;
-  static_cast<T*>(p.dw)[col] = from_float<T>(sh[0][0][lane]);
-  static_cast<T*>(p.db)[col] = from_float<T>(sh[1][0][lane]);
+  for (int q = 0; q < 32; ++q) v += sh[part][q][lane];
+  // Sum k of the column, from warp k or from this warp's lanes.
+  const int k = WIDE ? part : lane / kCols;
+  if (!has) return;
+  if (k == 0) static_cast<T*>(p.dw)[col] = from_float<T>(v);
+  if (k == 1) static_cast<T*>(p.db)[col] = from_float<T>(v);
   if constexpr (BRANCH) {
-    const float pw = to_float(static_cast<const T*>(p.pw)[col]), pb = to_float(static_cast<const T*>(p.pb)[col]);
+    if (k < 2) return;
     const float g = to_float(static_cast<const T*>(p.gate)[col]);
-    static_cast<T*>(p.dgate)[col] = from_float<T>(pw * sh[2][0][lane] + pb * sh[3][0][lane]);
-    static_cast<T*>(p.dpw)[col] = from_float<T>(g * sh[2][0][lane]);
-    static_cast<T*>(p.dpb)[col] = from_float<T>(g * sh[3][0][lane]);
+    if (k == 3) {
+      static_cast<T*>(p.dpb)[col] = from_float<T>(g * v);
+      return;
+    }
+    // k = 2: Q once more, in the same order.
+    float Q = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) Q += WIDE ? sh[kEach - 1][q][lane] : sh[0][q][(lane + kCols) & 31];
+    const float pw = to_float(static_cast<const T*>(p.pw)[col]), pb = to_float(static_cast<const T*>(p.pb)[col]);
+    static_cast<T*>(p.dgate)[col] = from_float<T>(pw * v + pb * Q);
+    static_cast<T*>(p.dpw)[col] = from_float<T>(g * v);
   }
 }
 
@@ -770,7 +781,9 @@ int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   f.parts = std::min(std::min(p.rows, most_ctas(kSmThreads / NT, smem)), std::max(p.rows / 4, 148));
   join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
   if (const int r = int(cudaGetLastError())) return r;
-  join_finish_kernel<T, BRANCH><<<unsigned((p.cols + 31) / 32), 1024, 0, s>>>(f);
+  constexpr bool kWide = NT * NV * 8 > 2048;
+  constexpr int kCols = kWide ? 32 : BRANCH ? 8 : 16;
+  join_finish_kernel<T, BRANCH, kWide><<<unsigned((p.cols + kCols - 1) / kCols), 1024, 0, s>>>(f);
   return int(cudaGetLastError());
 }
 template <typename T, bool VEC, bool BRANCH, bool PACKED>

@@ -31,9 +31,8 @@ namespace kernels {
 namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;  // of the merge and the gradient
 constexpr int kMaxTop = 32;       // alternatives a row: one sorted list per warp
-constexpr int kCandidates = 1024;  // 8 KB; more than that takes the selection by rounds
 constexpr int kUnroll = 4;
-constexpr int kRowThreads = 256, kRowCtas = 6;  // threads of a row's CTA, CTAs an SM takes at once
+constexpr int kSmThreads = 1536;  // of all CTAs on an SM, at 40 registers each
 constexpr float kLog2e = 1.44269504088896340736f;
 // e^d with d below this is zero in FP32; it also keeps 0 * (-inf) out of u.
 constexpr float kLowest = -200.f;
@@ -337,6 +336,7 @@ template <int NT>
 struct TopShared {
   static constexpr int W = NT / 32;
   Key lists[W][32];
+  static constexpr int kCandidates = 4 * NT;  // more than that takes the selection by rounds
   Key candidates[kCandidates];
   Key best[W];
   unsigned active[NT];
@@ -395,7 +395,7 @@ __device__ __forceinline__ bool fast_top(const Part<T>& part, float own, int k, 
   auto take = [&](float value, unsigned index) {
     if (value >= bound) {
       const unsigned at = atomicAdd(&sh.count, 1u);
-      if (at < kCandidates) sh.candidates[at] = make_key(value, index);
+      if (at < TopShared<NT>::kCandidates) sh.candidates[at] = make_key(value, index);
     }
   };
   // A warp for each active thread: its vectors are NT apart.
@@ -421,7 +421,7 @@ __device__ __forceinline__ bool fast_top(const Part<T>& part, float own, int k, 
   }
   __syncthreads();
   const unsigned n = sh.count;
-  if (n > kCandidates) return false;
+  if (n > TopShared<NT>::kCandidates) return false;
   if (warp == 0) sort_candidates(sh, n);
   return true;
 }
@@ -480,11 +480,11 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
   };
   visit([&](Key key) {
     const unsigned at = atomicAdd(&sh.count, 1u);
-    if (at < kCandidates) sh.candidates[at] = key;
+    if (at < TopShared<NT>::kCandidates) sh.candidates[at] = key;
   });
   __syncthreads();
   const unsigned n = sh.count;
-  if (n <= kCandidates) {
+  if (n <= TopShared<NT>::kCandidates) {
     if (warp == 0) sort_candidates(sh, n);
   } else {
     // Many candidates in few threads' vectors: the k largest one after another.
@@ -515,7 +515,7 @@ __device__ __forceinline__ void block_top(const Part<T>& part, Key own, int k, T
 
 // grid = rows * C CTAs in clusters of C; the cluster's CTAs take `chunk` columns each.
 template <typename T, bool TOP, int NT>
-__global__ void __launch_bounds__(NT, kRowCtas) score_kernel(const T* logits, int64_t ld, unsigned vocab,
+__global__ void __launch_bounds__(NT, kSmThreads / NT) score_kernel(const T* logits, int64_t ld, unsigned vocab,
                                                          const int64_t* targets, int64_t start,
                                                          int64_t vocab_total, unsigned chunk, Out o) {
   constexpr int W = NT / 32;
@@ -751,18 +751,36 @@ int launch_score(const void* logits, int64_t ld, unsigned vocab, const int64_t* 
   attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
-  config.numAttrs = 1;
+  config.numAttrs = C > 1 ? 1 : 0;
   return int(cudaLaunchKernelEx(&config, score_kernel<T, TOP, NT>, static_cast<const T*>(logits), ld, vocab, targets,
                                 start, vocab_total, chunk, o));
+}
+template <typename T, int NT>
+int score_threads(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
+                  int64_t vocab_total, const Out& o, unsigned C, cudaStream_t s) {
+  return o.k ? launch_score<T, true, NT>(logits, ld, vocab, targets, start, vocab_total, o, C, s)
+             : launch_score<T, false, NT>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
 }
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
-  // A row is split over a cluster while the rows alone leave SMs idle.
+  // A row is split over a cluster while the rows alone leave SMs idle (1 row of 50304: 9.8 us
+  // on four CTAs, 11.6 us on one; with more rows than SMs the split only costs).
   unsigned C = 1;
-  while (C < 8 && int64_t(o.rows) * C * 2 <= 148 * kRowCtas && vocab / (2 * C) >= 4096) C *= 2;
-  return o.k ? launch_score<T, true, kRowThreads>(logits, ld, vocab, targets, start, vocab_total, o, C, s)
-             : launch_score<T, false, kRowThreads>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
+  while (C < 4 && int64_t(o.rows) * C * 2 <= 148 && vocab / (2 * C) >= 4096) C *= 2;
+  // Threads of a row's CTA: what a row costs beside its loads (joining the threads' sums
+  // and lists) grows with them, its latency falls.  Many rows take one for every twenty
+  // or so vectors, and four for every alternative, so that few candidates pass the bound.
+  // 8192 BF16 rows, 8 alternatives: 64 threads 42 us and 256 threads 76 us at 6288 columns,
+  // 227 and 161 us at 50304.
+  int nt = 256;
+  if (o.rows > 148 * 4) {
+    const unsigned vectors = vocab / Vec<T>::kN;
+    while (nt > 64 && vectors < unsigned(nt) * 20 && nt / 2 >= 4 * o.k) nt /= 2;
+  }
+  if (nt == 64) return score_threads<T, 64>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
+  if (nt == 128) return score_threads<T, 128>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
+  return score_threads<T, 256>(logits, ld, vocab, targets, start, vocab_total, o, C, s);
 }
 template <typename T>
 int score_bwd_typed(const void* logits, int64_t ld, int rows, unsigned vocab, const int64_t* targets, int64_t start,
