@@ -34,8 +34,8 @@ __device__ __forceinline__ unsigned short encode2(float a, float b, float invers
   return __nv_cvt_float2_to_fp8x2(make_float2(a * inverse, b * inverse), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Eight values to p (on a 16-byte boundary).
-__device__ __forceinline__ void put8(__nv_bfloat16* p, const Two* v) {
+// A piece of 16 bytes to p.
+__device__ __forceinline__ void put(__nv_bfloat16* p, const Two* v) {
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -45,29 +45,22 @@ __device__ __forceinline__ void put8(__nv_bfloat16* p, const Two* v) {
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void put8(float* p, const Two* v) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float2 a = both(v[2 * i]), b = both(v[2 * i + 1]);
-    reinterpret_cast<float4*>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
-  }
+__device__ __forceinline__ void put(float* p, const Two* v) {
+  const float2 a = both(v[0]), b = both(v[1]);
+  *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Largest magnitude of eight values, and whether all are finite.
-__device__ __forceinline__ float largest(const Eight<__nv_bfloat16>& e) {
+// Largest magnitude of a piece, NaN if it holds one.
+__device__ __forceinline__ float largest(const Piece<__nv_bfloat16>& e) {
   // Magnitudes of BF16 pairs order like unsigned 16-bit numbers.
-  const uint4& r = e.raw[0];
+  const uint4& r = e.raw;
   constexpr unsigned kAbs = 0x7fff7fffu;
   const unsigned m = __vmaxu2(__vmaxu2(r.x & kAbs, r.y & kAbs), __vmaxu2(r.z & kAbs, r.w & kAbs));
   return __uint_as_float(max(m & 0xffff0000u, m << 16));
 }
-__device__ __forceinline__ float largest(const Eight<float>& e) {
-  float m = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    m = max_nan(max_nan(max_nan(m, fabsf(__uint_as_float(e.raw[h].x))), fabsf(__uint_as_float(e.raw[h].y))),
-                max_nan(fabsf(__uint_as_float(e.raw[h].z)), fabsf(__uint_as_float(e.raw[h].w))));
-  return m;
+__device__ __forceinline__ float largest(const Piece<float>& e) {
+  return max_nan(max_nan(fabsf(__uint_as_float(e.raw.x)), fabsf(__uint_as_float(e.raw.y))),
+                 max_nan(fabsf(__uint_as_float(e.raw.z)), fabsf(__uint_as_float(e.raw.w))));
 }
 
 // The exponent byte of a group from its values' largest magnitude `amax` over the
@@ -97,39 +90,48 @@ __device__ __forceinline__ unsigned settle(float* v, float amax) {
 }
 __device__ __forceinline__ float inverse_unit(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Eight lanes per group; a lane has eight columns of each half, so that every
-// load and store of a group is one contiguous piece.
+// Eight lanes per group.  A lane has a piece of 16 bytes of every eighth, so that each
+// load and store of a group's lanes is one contiguous stretch (pieces of a lane side by
+// side would move every sector twice).
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsigned char* data, int cols,
                                                    unsigned groups, unsigned items) {
+  using P = Piece<T>;
+  constexpr int kPieces = 16 / P::kN;
   const int lane = threadIdx.x & 7;
   const unsigned item = blockIdx.x * 32u + threadIdx.x / 8u;
   const bool live = item < items;
   const unsigned row = live ? item / groups : 0u, group = live ? item - row * groups : 0u;
-  const int col = int(group) * kPackGroup + lane * 8;
-  Eight<T> e[2];
+  const int col = int(group) * kPackGroup + lane * P::kN;
+  P e[kPieces];
+  float v[16], amax = 0.f;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < int(sizeof(T) / 2); ++i) e[h].raw[i] = make_uint4(0, 0, 0, 0);
-    if (live && col + h * 64 < cols) e[h].load_once(x + int64_t(row) * ld + col + h * 64);
+  for (int h = 0; h < kPieces; ++h) {
+    e[h].raw = make_uint4(0, 0, 0, 0);
+    if (live && col + h * 8 * P::kN < cols) e[h].load_once(x + int64_t(row) * ld + col + h * 8 * P::kN);
   }
-  float v[16];
-  e[0].get(v);
-  e[1].get(v + 8);
-  const unsigned byte = settle<8, 16>(v, max_nan(largest(e[0]), largest(e[1])));
+#pragma unroll
+  for (int h = 0; h < kPieces; ++h) {
+    e[h].get(v + h * P::kN);
+    amax = max_nan(amax, largest(e[h]));
+  }
+  const unsigned byte = settle<8, 16>(v, amax);
   if (!live) return;
   const float inverse = inverse_unit(byte);
   unsigned char* dst = data + int64_t(row) * pack_row_bytes(cols);
   const int code_bytes = int(pack_code_bytes(cols));
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (col + h * 64 >= code_bytes) break;
-    uint2 codes;
-    codes.x = encode2(v[h * 8], v[h * 8 + 1], inverse) | unsigned(encode2(v[h * 8 + 2], v[h * 8 + 3], inverse)) << 16;
-    codes.y = encode2(v[h * 8 + 4], v[h * 8 + 5], inverse) |
-              unsigned(encode2(v[h * 8 + 6], v[h * 8 + 7], inverse)) << 16;
-    *reinterpret_cast<uint2*>(dst + col + h * 64) = codes;
+  for (int h = 0; h < kPieces; ++h) {
+    if (col + h * 8 * P::kN >= code_bytes) break;
+    unsigned codes[P::kN / 4];
+#pragma unroll
+    for (int i = 0; i < P::kN / 4; ++i) {
+      const float* f = v + h * P::kN + i * 4;
+      codes[i] = encode2(f[0], f[1], inverse) | unsigned(encode2(f[2], f[3], inverse)) << 16;
+    }
+    unsigned char* to = dst + col + h * 8 * P::kN;
+    if constexpr (P::kN == 8) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+    else *reinterpret_cast<unsigned*>(to) = codes[0];
   }
   unsigned char* units = dst + code_bytes;
   if (lane == 0) units[group] = static_cast<unsigned char>(byte);
@@ -201,22 +203,30 @@ __device__ __forceinline__ float kept_gelu(float v, const float* table) {
   return v * table[(kTablePad + k + int(bits >> 31) * kTableHalf) * kCopies];
 }
 
-// Eight columns per thread and step; the next step's codes are loaded ahead.
+// As many columns per thread and step as fill 16 bytes of an output; the next step's
+// codes are loaded ahead.
 template <typename T, bool GELU>
 __global__ void __launch_bounds__(1024, 2) unpack_kernel(const unsigned char* data, T* out, T* act, int cols,
                                                          unsigned segments, unsigned items) {
   extern __shared__ __align__(16) float table[];
+  constexpr int kN = Piece<T>::kN;
   const unsigned row_bytes = unsigned(pack_row_bytes(cols)), code_bytes = unsigned(pack_code_bytes(cols));
   const unsigned stride = gridDim.x * 1024u, row_step = stride / segments, step = stride - row_step * segments;
   unsigned item = blockIdx.x * 1024u + threadIdx.x;
   unsigned row = item / segments, seg = item - row * segments;
-  uint2 codes = make_uint2(0, 0);
+  unsigned codes[kN / 4] = {};
   unsigned byte = 1;
   auto load = [&] {
     if (item < items) {
       const unsigned char* src = data + int64_t(row) * row_bytes;
-      codes = *reinterpret_cast<const uint2*>(src + seg * 8);
-      byte = src[code_bytes + seg / (kPackGroup / 8)];
+      if constexpr (kN == 8) {
+        const uint2 c = *reinterpret_cast<const uint2*>(src + seg * 8);
+        codes[0] = c.x;
+        codes[1] = c.y;
+      } else {
+        codes[0] = *reinterpret_cast<const unsigned*>(src + seg * 4);
+      }
+      byte = src[code_bytes + seg / (kPackGroup / kN)];
     }
   };
   load();
@@ -225,9 +235,11 @@ __global__ void __launch_bounds__(1024, 2) unpack_kernel(const unsigned char* da
     __syncthreads();
   }
   while (item < items) {
-    const uint2 now = codes;
+    unsigned now[kN / 4];
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i) now[i] = codes[i];
     const unsigned unit_byte = byte;
-    const int64_t at = int64_t(row) * cols + seg * 8;
+    const int64_t at = int64_t(row) * cols + seg * kN;
     item += stride;
     row += row_step;
     seg += step;
@@ -241,10 +253,10 @@ __global__ void __launch_bounds__(1024, 2) unpack_kernel(const unsigned char* da
     const bool window = unit_byte - 112u <= 14u;
     const char* place = reinterpret_cast<const char*>(
         table + (kTablePad + 8 * (int(unit_byte) - 127 + 9)) * kCopies + (threadIdx.x & (kCopies - 1)));
-    Two v[4], a[4];
+    Two v[kN / 2], a[kN / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned word = i < 2 ? now.x : now.y;
+    for (int i = 0; i < kN / 2; ++i) {
+      const unsigned word = now[i / 2];
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(i & 1 ? word >> 16 : word & 0xffffu), __NV_E4M3);
       const float2 f = __half22float2(__half2(h));
       v[i] = two_mul(two(f.x, f.y), two(unit, unit));
@@ -258,13 +270,13 @@ __global__ void __launch_bounds__(1024, 2) unpack_kernel(const unsigned char* da
     }
     if (GELU && !window) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kN / 2; ++i) {
         const float2 f = both(v[i]);
         a[i] = two(kept_gelu(f.x, table), kept_gelu(f.y, table));
       }
     }
-    put8(out + at, v);
-    if (GELU) put8(act + at, a);
+    put(out + at, v);
+    if (GELU) put(act + at, a);
   }
 }
 
@@ -318,7 +330,7 @@ int pack_typed(const void* x, int64_t ld, void* data, int64_t rows, int64_t cols
 template <typename T, bool GELU>
 int unpack_typed(const void* data, void* out, void* act, int64_t rows, int64_t cols, cudaStream_t s) {
   const bool vec = cols % 8 == 0 && aligned16(out) && (!GELU || aligned16(act));
-  const int64_t segments = vec ? cols / 8 : (cols + 511) / 512, items = rows * segments;
+  const int64_t segments = vec ? cols / Piece<T>::kN : (cols + 511) / 512, items = rows * segments;
   if (items > 0x7fffffff) return -1;
   auto launch = [&](auto kernel, int per_cta, int threads, int most, int smem) {
     const int64_t ctas = (items + per_cta - 1) / per_cta;

@@ -22,8 +22,8 @@
 // the next ones (two forward, one backward) on their way into shared memory (cp.async)
 // while it works on one, so loads are in flight all the time and no register holds them.
 //   Vector form (width a multiple of 8, rows on 16-byte boundaries): a thread has
-// eight consecutive columns at a time and copies what it will read itself, so it
-// waits for its own copies alone.
+// pieces of 16 bytes and copies what it will read itself, so it waits for its own
+// copies alone.
 //   Otherwise (odd widths, views) the CTA copies the 16-byte pieces that cover the
 // row, and threads read single values at the row's offset, columns a CTA's width
 // apart: one barrier more a row.
@@ -158,16 +158,20 @@ struct Matrix {
   int64_t ld;
 };
 
-// A thread's columns, eight together (VEC) or a CTA's width apart, and a matrix's row: copied to `region` of shared memory, read from there, or written.
+// A thread's columns, in groups of eight, and a matrix's row: copied to `region` of
+// shared memory, read from there, or written.  Vector form: a group is one or two
+// pieces of 16 bytes, and neighbouring threads have neighbouring pieces, so that every
+// access of a warp is contiguous; otherwise columns a CTA's width apart.
 template <typename T, int NT, int NV, bool VEC>
 struct Tile {
-  static constexpr int kPieces = int(sizeof(T)) / 2;
+  static constexpr int kPieces = int(sizeof(T)) / 2, kPer = 8 / kPieces;
   static __host__ __device__ constexpr int bytes(int cols) {
     return VEC ? NT * NV * 8 * int(sizeof(T)) : ((cols * int(sizeof(T)) + 15) / 16 + 1) * 16;
   }
   static __device__ __forceinline__ int column(int g, int i = 0) {
-    return VEC ? (g * NT + int(threadIdx.x)) * 8 + i : (g * 8 + i) * NT + int(threadIdx.x);
+    return VEC ? ((g * kPieces + i / kPer) * NT + int(threadIdx.x)) * kPer + i % kPer : (g * 8 + i) * NT + int(threadIdx.x);
   }
+  static __device__ __forceinline__ int piece(int g, int i) { return column(g, i * kPer); }
   // Not vectors: the eight columns of group g at p.
   static __device__ __forceinline__ void singles(const T* p, int cols, int g, Two* v) {
     float f[8];
@@ -183,13 +187,11 @@ struct Tile {
     const T* r = row_of(m, row);
     if constexpr (VEC) {
 #pragma unroll
-      for (int g = 0; g < NV; ++g) {
-        if (column(g) >= cols) continue;
+      for (int g = 0; g < NV; ++g)
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
-          copy_async<16>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16,
-                         reinterpret_cast<const uint4*>(r + column(g)) + i);
-      }
+          if (piece(g, i) < cols)
+            copy_async<16>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16, r + piece(g, i));
     } else {
       // Pieces that reach past the matrix's first or last value are copied value by value.
       const uintptr_t at = reinterpret_cast<uintptr_t>(r) & ~uintptr_t(15);
@@ -229,14 +231,13 @@ struct Tile {
     __device__ __forceinline__ void load(const void* base, int cols, bool zeros = false) {
       if constexpr (VEC) {
 #pragma unroll
-        for (int g = 0; g < NV; ++g) {
-          const int c = column(g) < cols ? column(g) : 0;
+        for (int g = 0; g < NV; ++g)
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            raw[g][i] = ld_vector(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + c) + i);
-            if (zeros && column(g) >= cols) raw[g][i] = make_uint4(0, 0, 0, 0);
+            const bool has = piece(g, i) < cols;
+            raw[g][i] = ld_vector(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + (has ? piece(g, i) : 0)));
+            if (zeros && !has) raw[g][i] = make_uint4(0, 0, 0, 0);
           }
-        }
       }
     }
     __device__ __forceinline__ void get(const void* base, int cols, int g, Two* v) const {
@@ -251,7 +252,7 @@ struct Tile {
       uint4 raw[kPieces];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        raw[i] = column(g) < cols ? reinterpret_cast<const uint4*>(p + column(g))[i] : make_uint4(0, 0, 0, 0);
+        raw[i] = piece(g, i) < cols ? *reinterpret_cast<const uint4*>(p + piece(g, i)) : make_uint4(0, 0, 0, 0);
       Conv<T>::get(raw, v);
     } else {
       singles(p, cols, g, v);
@@ -260,11 +261,11 @@ struct Tile {
   static __device__ __forceinline__ void store(void* base, int64_t ld, int64_t row, int cols, int g, const Two* v) {
     T* p = static_cast<T*>(base) + row * ld;
     if constexpr (VEC) {
-      if (column(g) >= cols) return;
       uint4 raw[kPieces];
       Conv<T>::put(v, raw);
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p + column(g))[i] = raw[i];
+      for (int i = 0; i < kPieces; ++i)
+        if (piece(g, i) < cols) *reinterpret_cast<uint4*>(p + piece(g, i)) = raw[i];
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -274,25 +275,41 @@ struct Tile {
       }
     }
   }
+  // FP32 sums over the rows, at the same columns.
+  static __device__ __forceinline__ void store_sums(float* p, int cols, int g, const Two* v) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const float2 a = both(v[i]), b = both(v[i + 1]);
+      if constexpr (VEC) {
+        if (column(g, 2 * i) < cols) *reinterpret_cast<float4*>(p + column(g, 2 * i)) = make_float4(a.x, a.y, b.x, b.y);
+      } else {
+        if (column(g, 2 * i) < cols) p[column(g, 2 * i)] = a.x;
+        if (column(g, 2 * i + 1) < cols) p[column(g, 2 * i + 1)] = a.y;
+        if (column(g, 2 * i + 2) < cols) p[column(g, 2 * i + 2)] = b.x;
+        if (column(g, 2 * i + 3) < cols) p[column(g, 2 * i + 3)] = b.y;
+      }
+    }
+  }
 };
 
-// The same of packed rows.  Vector form: eight codes and the four exponent bytes with
-// the group's own among them; otherwise the whole row (it starts on a boundary).
-template <int NT, int NV, bool VEC>
+// The same columns of packed rows.  Vector form: a piece's codes and the four exponent
+// bytes with its own among them; otherwise the whole row (it starts on a boundary).
+template <typename T, int NT, int NV, bool VEC>
 struct PackedTile {
-  using C = Tile<float, NT, NV, VEC>;
+  using C = Tile<T, NT, NV, VEC>;
+  static constexpr int kPieces = C::kPieces;
   static __host__ __device__ constexpr int bytes(int cols) {
-    return VEC ? NT * NV * 12 : int(pack_row_bytes(cols));
+    return VEC ? NT * NV * (8 + 4 * kPieces) : int(pack_row_bytes(cols));
   }
   static __device__ __forceinline__ void fetch(char* region, const Matrix& m, int64_t row, int, int cols) {
     const char* r = static_cast<const char*>(m.data) + row * m.ld;
     if constexpr (VEC) {
 #pragma unroll
-      for (int g = 0; g < NV; ++g) {
-        const int col = C::column(g);
+      for (int k = 0; k < NV * kPieces; ++k) {
+        const int col = C::piece(k / kPieces, k % kPieces);
         if (col >= cols) continue;
-        copy_async<8>(region + (g * NT + threadIdx.x) * 8, r + col);
-        copy_async<4>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4,
+        copy_async<C::kPer>(region + (k * NT + threadIdx.x) * C::kPer, r + col);
+        copy_async<4>(region + NT * NV * 8 + (k * NT + threadIdx.x) * 4,
                       r + pack_code_bytes(cols) + (col / kPackGroup & ~3));
       }
     } else {
@@ -302,9 +319,19 @@ struct PackedTile {
   static __device__ __forceinline__ void get(const char* region, const Matrix&, int64_t, int cols, int g, Two* v) {
     float f[8];
     if constexpr (VEC) {
-      const uint2 codes = *reinterpret_cast<const uint2*>(region + (g * NT + threadIdx.x) * 8);
-      const unsigned four = *reinterpret_cast<const unsigned*>(region + NT * NV * 8 + (g * NT + threadIdx.x) * 4);
-      decode8(codes, pack_unit(four >> (8 * (C::column(g) / kPackGroup & 3)) & 0xffu), f);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int k = g * kPieces + i;
+        const unsigned four = *reinterpret_cast<const unsigned*>(region + NT * NV * 8 + (k * NT + threadIdx.x) * 4);
+        const float unit = pack_unit(four >> (8 * (C::piece(g, i) / kPackGroup & 3)) & 0xffu);
+        const unsigned* codes = reinterpret_cast<const unsigned*>(region + (k * NT + threadIdx.x) * C::kPer);
+        if constexpr (C::kPer == 8) {
+          decode8(*reinterpret_cast<const uint2*>(codes), unit, f);
+        } else {
+          decode2(*codes & 0xffffu, unit, f + i * 4);
+          decode2(*codes >> 16, unit, f + i * 4 + 2);
+        }
+      }
     } else {
       const unsigned char* r = reinterpret_cast<const unsigned char*>(region);
 #pragma unroll
@@ -385,17 +412,20 @@ __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, floa
   s = 0;
 #pragma unroll
   for (int g = 0; g < NV; ++g) {
-    Two q = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      Two d = two_add(v[g * 4 + i], minus);
-      if (!VEC) {  // single columns may lie past the width
-        const float2 f = both(d);
-        d = two(C::column(g, 2 * i) < p.cols ? f.x : 0.f, C::column(g, 2 * i + 1) < p.cols ? f.y : 0.f);
+    for (int k = 0; k < C::kPieces; ++k) {
+      Two q = 0;
+#pragma unroll
+      for (int i = k * C::kPer / 2; i < (k + 1) * C::kPer / 2; ++i) {
+        Two d = two_add(v[g * 4 + i], minus);
+        if (!VEC) {  // single columns may lie past the width
+          const float2 f = both(d);
+          d = two(C::column(g, 2 * i) < p.cols ? f.x : 0.f, C::column(g, 2 * i + 1) < p.cols ? f.y : 0.f);
+        }
+        q = two_fma(d, d, q);
       }
-      q = two_fma(d, d, q);
+      if (!VEC || C::piece(g, k) < p.cols) s = two_add(s, q);
     }
-    if (!VEC || C::column(g) < p.cols) s = two_add(s, q);
   }
   const float var = cta_sum<NT>(total(s), sh + 16) * p.inverse;
   return make_float2(mean, rsqrtf(var + p.eps));
@@ -478,7 +508,7 @@ struct JoinBwd {
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 struct BwdTiles {
   using C = Tile<T, NT, NV, VEC>;
-  using K = std::conditional_t<PACKED, PackedTile<NT, NV, VEC>, C>;
+  using K = std::conditional_t<PACKED, PackedTile<T, NT, NV, VEC>, C>;
   static __host__ __device__ constexpr int bytes(int cols) { return 2 * C::bytes(cols) + (BRANCH ? 2 : 1) * K::bytes(cols); }
 };
 
@@ -664,15 +694,14 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) join_bwd_kernel(JoinBwd p
           }
         }
       });
-  using F = Tile<float, NT, NV, VEC>;
   float* out = p.sums + int64_t(blockIdx.x) * (BRANCH ? 4 : 2) * p.cols;
 #pragma unroll
   for (int g = 0; g < NV; ++g) {
-    F::store(out, 0, 0, p.cols, g, dw + g * 4);
-    F::store(out + p.cols, 0, 0, p.cols, g, db + g * 4);
+    C::store_sums(out, p.cols, g, dw + g * 4);
+    C::store_sums(out + p.cols, p.cols, g, db + g * 4);
     if constexpr (BRANCH) {
-      F::store(out + 2 * int64_t(p.cols), 0, 0, p.cols, g, P + g * 4);
-      F::store(out + 3 * int64_t(p.cols), 0, 0, p.cols, g, Q + g * 4);
+      C::store_sums(out + 2 * int64_t(p.cols), p.cols, g, P + g * 4);
+      C::store_sums(out + 3 * int64_t(p.cols), p.cols, g, Q + g * 4);
     }
   }
 }
@@ -765,16 +794,18 @@ template <typename T, bool VEC>
 int fwd_pick(const JoinFwd& p, cudaStream_t s) {
   if (p.cols <= 256) return fwd_launch<T, 32, 1, VEC>(p, s);
   if (p.cols <= 1024) return fwd_launch<T, 128, 1, VEC>(p, s);
-  if (p.cols <= 2048) return fwd_launch<T, 128, 2, VEC>(p, s);
-  if (p.cols <= 4096) return fwd_launch<T, 128, 4, VEC>(p, s);
-  return fwd_launch<T, 256, 4, VEC>(p, s);
+  // FP32 rows leave room for half as many CTAs, so they have twice the threads.
+  constexpr int kMore = sizeof(T) == 4 ? 2 : 1;
+  if (p.cols <= 2048) return fwd_launch<T, 128 * kMore, 2 / kMore, VEC>(p, s);
+  if (p.cols <= 4096) return fwd_launch<T, 128 * kMore, 4 / kMore, VEC>(p, s);
+  return fwd_launch<T, 256 * kMore, 4 / kMore, VEC>(p, s);
 }
 
 // The gradient's CTAs: as many as fit, but four rows each where that leaves every SM one.
 template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   // Two rows of the widest FP32 tensors are more than an SM holds.
-  constexpr int kRows = sizeof(T) == 4 && NT == 512 ? 1 : kBwdStages;
+  constexpr int kRows = sizeof(T) == 4 && NT * NV == 1024 ? 1 : kBwdStages;
   const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
@@ -790,8 +821,10 @@ template <typename T, bool VEC, bool BRANCH, bool PACKED>
 int bwd_pick(const JoinBwd& p, const JoinFinish& f, cudaStream_t s) {
   if (p.cols <= 256) return bwd_launch<T, 32, 1, VEC, BRANCH, PACKED>(p, f, s);
   if (p.cols <= 1024) return bwd_launch<T, 128, 1, VEC, BRANCH, PACKED>(p, f, s);
-  if (p.cols <= 2048) return bwd_launch<T, 128, 2, VEC, BRANCH, PACKED>(p, f, s);
-  if (p.cols <= 4096) return bwd_launch<T, 256, 2, VEC, BRANCH, PACKED>(p, f, s);
+  // FP32 rows leave room for half as many CTAs, so they have twice the threads.
+  constexpr bool kLong = sizeof(T) == 4 && !PACKED;
+  if (p.cols <= 2048) return bwd_launch<T, kLong ? 256 : 128, kLong ? 1 : 2, VEC, BRANCH, PACKED>(p, f, s);
+  if (p.cols <= 4096) return bwd_launch<T, kLong ? 512 : 256, kLong ? 1 : 2, VEC, BRANCH, PACKED>(p, f, s);
   return bwd_launch<T, 512, 2, VEC, BRANCH, PACKED>(p, f, s);
 }
 }  // namespace

@@ -21,23 +21,20 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 
-// Eight consecutive values as they lie in memory; p is 16-byte aligned.
+// 16 bytes of values as they lie in memory, read once, past L1.
 template <typename T>
-struct Eight {
-  uint4 raw[sizeof(T) / 2];
-  // Values that are read once pass by L1.
+struct Piece {
+  static constexpr int kN = 16 / int(sizeof(T));
+  uint4 raw;
   __device__ __forceinline__ void load_once(const T* p) {
-#pragma unroll
-    for (int i = 0; i < int(sizeof(T) / 2); ++i) {
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w)
-                   : "l"(reinterpret_cast<const uint4*>(p) + i));
-    }
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w)
+                 : "l"(reinterpret_cast<const uint4*>(p)));
   }
   __device__ __forceinline__ void get(float* v) const {
-    const T* h = reinterpret_cast<const T*>(raw);
+    const T* h = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(h[i]);
+    for (int i = 0; i < kN; ++i) v[i] = to_float(h[i]);
   }
 };
 
