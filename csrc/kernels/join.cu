@@ -162,16 +162,17 @@ struct Matrix {
 // shared memory, read from there, or written.  Vector form: a group is one or two
 // pieces of 16 bytes, and neighbouring threads have neighbouring pieces, so that every
 // access of a warp is contiguous; otherwise columns a CTA's width apart.
-template <typename T, int NT, int NV, bool VEC>
+template <typename T, int NT, int NV, int FORM>
 struct Tile {
   static constexpr int kPieces = int(sizeof(T)) / 2, kPer = 8 / kPieces;
   static __host__ __device__ constexpr int bytes(int cols) {
-    return VEC ? NT * NV * 8 * int(sizeof(T)) : ((cols * int(sizeof(T)) + 15) / 16 + 1) * 16;
+    return FORM ? NT * NV * 8 * int(sizeof(T)) : ((cols * int(sizeof(T)) + 15) / 16 + 1) * 16;
   }
   static __device__ __forceinline__ int column(int g, int i = 0) {
-    return VEC ? ((g * kPieces + i / kPer) * NT + int(threadIdx.x)) * kPer + i % kPer : (g * 8 + i) * NT + int(threadIdx.x);
+    return FORM ? ((g * kPieces + i / kPer) * NT + int(threadIdx.x)) * kPer + i % kPer : (g * 8 + i) * NT + int(threadIdx.x);
   }
   static __device__ __forceinline__ int piece(int g, int i) { return column(g, i * kPer); }
+  static __device__ __forceinline__ bool has(int g, int i, int cols) { return FORM == 2 || piece(g, i) < cols; }
   // Not vectors: the eight columns of group g at p.
   static __device__ __forceinline__ void singles(const T* p, int cols, int g, Two* v) {
     float f[8];
@@ -185,12 +186,12 @@ struct Tile {
   }
   static __device__ __forceinline__ void fetch(char* region, const Matrix& m, int64_t row, int rows, int cols) {
     const T* r = row_of(m, row);
-    if constexpr (VEC) {
+    if constexpr (FORM) {
 #pragma unroll
       for (int g = 0; g < NV; ++g)
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
-          if (piece(g, i) < cols)
+          if (has(g, i, cols))
             copy_async<16>(region + ((g * kPieces + i) * NT + threadIdx.x) * 16, r + piece(g, i));
     } else {
       // Pieces that reach past the matrix's first or last value are copied value by value.
@@ -212,7 +213,7 @@ struct Tile {
   }
   // Group g of the row in `region`; zeros past the width (`clear`).
   static __device__ __forceinline__ void get(const char* region, const Matrix& m, int64_t row, int cols, int g, Two* v) {
-    if constexpr (VEC) {
+    if constexpr (FORM) {
       uint4 raw[kPieces];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
@@ -227,32 +228,32 @@ struct Tile {
   // the loads' latency and the reduction's pass together.  Past the width it holds the
   // first columns' values, or zeros where they are asked for.
   struct Vector {
-    uint4 raw[VEC ? NV : 1][kPieces];
+    uint4 raw[FORM ? NV : 1][kPieces];
     __device__ __forceinline__ void load(const void* base, int cols, bool zeros = false) {
-      if constexpr (VEC) {
+      if constexpr (FORM) {
 #pragma unroll
         for (int g = 0; g < NV; ++g)
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            const bool has = piece(g, i) < cols;
-            raw[g][i] = ld_vector(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + (has ? piece(g, i) : 0)));
-            if (zeros && !has) raw[g][i] = make_uint4(0, 0, 0, 0);
+            const bool in = has(g, i, cols);
+            raw[g][i] = ld_vector(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + (in ? piece(g, i) : 0)));
+            if (zeros && !in) raw[g][i] = make_uint4(0, 0, 0, 0);
           }
       }
     }
     __device__ __forceinline__ void get(const void* base, int cols, int g, Two* v) const {
-      if constexpr (VEC) Conv<T>::get(raw[g], v);
+      if constexpr (FORM) Conv<T>::get(raw[g], v);
       else singles(static_cast<const T*>(base), cols, g, v);
     }
   };
   // One group of such a vector, where it is needed.
   static __device__ __forceinline__ void group(const void* base, int cols, int g, Two* v) {
     const T* p = static_cast<const T*>(base);
-    if constexpr (VEC) {
+    if constexpr (FORM) {
       uint4 raw[kPieces];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        raw[i] = piece(g, i) < cols ? *reinterpret_cast<const uint4*>(p + piece(g, i)) : make_uint4(0, 0, 0, 0);
+        raw[i] = has(g, i, cols) ? *reinterpret_cast<const uint4*>(p + piece(g, i)) : make_uint4(0, 0, 0, 0);
       Conv<T>::get(raw, v);
     } else {
       singles(p, cols, g, v);
@@ -260,12 +261,12 @@ struct Tile {
   }
   static __device__ __forceinline__ void store(void* base, int64_t ld, int64_t row, int cols, int g, const Two* v) {
     T* p = static_cast<T*>(base) + row * ld;
-    if constexpr (VEC) {
+    if constexpr (FORM) {
       uint4 raw[kPieces];
       Conv<T>::put(v, raw);
 #pragma unroll
       for (int i = 0; i < kPieces; ++i)
-        if (piece(g, i) < cols) *reinterpret_cast<uint4*>(p + piece(g, i)) = raw[i];
+        if (has(g, i, cols)) *reinterpret_cast<uint4*>(p + piece(g, i)) = raw[i];
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -280,8 +281,8 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < 4; i += 2) {
       const float2 a = both(v[i]), b = both(v[i + 1]);
-      if constexpr (VEC) {
-        if (column(g, 2 * i) < cols) *reinterpret_cast<float4*>(p + column(g, 2 * i)) = make_float4(a.x, a.y, b.x, b.y);
+      if constexpr (FORM) {
+        if (has(g, 2 * i / kPer, cols)) *reinterpret_cast<float4*>(p + column(g, 2 * i)) = make_float4(a.x, a.y, b.x, b.y);
       } else {
         if (column(g, 2 * i) < cols) p[column(g, 2 * i)] = a.x;
         if (column(g, 2 * i + 1) < cols) p[column(g, 2 * i + 1)] = a.y;
@@ -294,23 +295,24 @@ struct Tile {
 
 // The same columns of packed rows.  Vector form: a piece's codes and the four exponent
 // bytes with its own among them; otherwise the whole row (it starts on a boundary).
-template <typename T, int NT, int NV, bool VEC>
+template <typename T, int NT, int NV, int FORM>
 struct PackedTile {
-  using C = Tile<T, NT, NV, VEC>;
+  using C = Tile<T, NT, NV, FORM>;
   static constexpr int kPieces = C::kPieces;
   static __host__ __device__ constexpr int bytes(int cols) {
-    return VEC ? NT * NV * (8 + 4 * kPieces) : int(pack_row_bytes(cols));
+    return FORM ? NT * NV * (8 + 4 * kPieces) : int(pack_row_bytes(cols));
   }
   static __device__ __forceinline__ void fetch(char* region, const Matrix& m, int64_t row, int, int cols) {
     const char* r = static_cast<const char*>(m.data) + row * m.ld;
-    if constexpr (VEC) {
+    if constexpr (FORM) {
 #pragma unroll
       for (int k = 0; k < NV * kPieces; ++k) {
         const int col = C::piece(k / kPieces, k % kPieces);
-        if (col >= cols) continue;
-        copy_async<C::kPer>(region + (k * NT + threadIdx.x) * C::kPer, r + col);
-        copy_async<4>(region + NT * NV * 8 + (k * NT + threadIdx.x) * 4,
-                      r + pack_code_bytes(cols) + (col / kPackGroup & ~3));
+        if (C::has(k / kPieces, k % kPieces, cols)) {
+          copy_async<C::kPer>(region + (k * NT + threadIdx.x) * C::kPer, r + col);
+          copy_async<4>(region + NT * NV * 8 + (k * NT + threadIdx.x) * 4,
+                        r + pack_code_bytes(cols) + (col / kPackGroup & ~3));
+        }
       }
     } else {
       for (int i = threadIdx.x; i < int(pack_row_bytes(cols)) / 16; i += NT) copy_async<16>(region + i * 16, r + i * 16);
@@ -318,7 +320,7 @@ struct PackedTile {
   }
   static __device__ __forceinline__ void get(const char* region, const Matrix&, int64_t, int cols, int g, Two* v) {
     float f[8];
-    if constexpr (VEC) {
+    if constexpr (FORM) {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int k = g * kPieces + i;
@@ -347,9 +349,9 @@ struct PackedTile {
 
 // Vector form: nothing is copied to the places of columns past the width, and what
 // is read from there is zero.
-template <int NT, bool VEC>
-__device__ __forceinline__ void clear(char* ring, int bytes, bool whole) {
-  if (VEC && !whole) {
+template <int NT, int FORM>
+__device__ __forceinline__ void clear(char* ring, int bytes) {
+  if (FORM == 1) {
     for (int i = threadIdx.x * 16; i < bytes; i += NT * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();  // other threads' places were cleared here too
   }
@@ -357,16 +359,16 @@ __device__ __forceinline__ void clear(char* ring, int bytes, bool whole) {
 
 // Walks over a CTA's rows with the next ones on their way: fetch(row, stage) starts
 // the copies of a row, work(row, stage) has them in place.
-template <int NT, bool VEC, int STAGES, typename Fetch, typename Work>
+template <int NT, int FORM, int STAGES, typename Fetch, typename Work>
 __device__ __forceinline__ void walk(int rows, Fetch&& fetch, Work&& work) {
   const int64_t step = gridDim.x;
   if constexpr (STAGES == 1) {
     for (int64_t row = blockIdx.x; row < rows; row += step) {
-      if constexpr (!VEC) __syncthreads();  // the last row has been read
+      if constexpr (!FORM) __syncthreads();  // the last row has been read
       fetch(row, 0);
       copies_commit();
       copies_wait<0>();
-      if constexpr (!VEC) __syncthreads();
+      if constexpr (!FORM) __syncthreads();
       work(row, 0);
     }
   } else {
@@ -380,7 +382,7 @@ __device__ __forceinline__ void walk(int rows, Fetch&& fetch, Work&& work) {
     for (int64_t row = blockIdx.x; row < rows; row += step) {
       copies_wait<STAGES - 2>();
       // Other threads' copies are in place, and the stage filled next has been read by all.
-      if constexpr (!VEC) __syncthreads();
+      if constexpr (!FORM) __syncthreads();
       const int64_t ahead = row + (STAGES - 1) * step;
       if (ahead < rows) fetch(ahead, stage == 0 ? STAGES - 1 : stage - 1);
       copies_commit();
@@ -402,7 +404,7 @@ struct JoinFwd {
 };
 
 // Mean and reciprocal deviation of a row: two passes over registers.
-template <int NT, int NV, bool VEC, typename C>
+template <int NT, int NV, int FORM, typename C>
 __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, float* sh) {
   Two s = 0;
 #pragma unroll
@@ -418,27 +420,27 @@ __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, floa
 #pragma unroll
       for (int i = k * C::kPer / 2; i < (k + 1) * C::kPer / 2; ++i) {
         Two d = two_add(v[g * 4 + i], minus);
-        if (!VEC) {  // single columns may lie past the width
+        if (!FORM) {  // single columns may lie past the width
           const float2 f = both(d);
           d = two(C::column(g, 2 * i) < p.cols ? f.x : 0.f, C::column(g, 2 * i + 1) < p.cols ? f.y : 0.f);
         }
         q = two_fma(d, d, q);
       }
-      if (!VEC || C::piece(g, k) < p.cols) s = two_add(s, q);
+      if (!FORM || C::has(g, k, p.cols)) s = two_add(s, q);
     }
   }
   const float var = cta_sum<NT>(total(s), sh + 16) * p.inverse;
   return make_float2(mean, rsqrtf(var + p.eps));
 }
 
-template <typename T, int NT, int NV, bool VEC, int STAGES>
+template <typename T, int NT, int NV, int FORM, int STAGES>
 __global__ void __launch_bounds__(NT, kSmThreads / NT) join_fwd_kernel(JoinFwd p) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float sh[64];
-  using C = Tile<T, NT, NV, VEC>;
+  using C = Tile<T, NT, NV, FORM>;
   const int bytes = C::bytes(p.cols);
-  clear<NT, VEC>(ring, STAGES * 2 * bytes, p.cols == NT * NV * 8);
-  walk<NT, VEC, STAGES>(
+  clear<NT, FORM>(ring, STAGES * 2 * bytes);
+  walk<NT, FORM, STAGES>(
       p.rows,
       [&](int64_t row, int stage) {
         C::fetch(ring + (2 * stage) * bytes, p.y, row, p.rows, p.cols);
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) join_fwd_kernel(JoinFwd p
         pw.load(p.pw, p.cols);
         pb.load(p.pb, p.cols);
         gate.load(p.gate, p.cols, true);  // columns past the width stay zero in u
-        float2 st = row_stats<NT, NV, VEC, C>(y, p, sh);
+        float2 st = row_stats<NT, NV, FORM, C>(y, p, sh);
         if (threadIdx.x == 0) {
           p.stats[row] = st.x;
           p.stats[p.rows + row] = st.y;
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) join_fwd_kernel(JoinFwd p
         }
         pw.load(p.w, p.cols);
         pb.load(p.b, p.cols);
-        st = row_stats<NT, NV, VEC, C>(y, p, sh + 32);
+        st = row_stats<NT, NV, FORM, C>(y, p, sh + 32);
         if (threadIdx.x == 0) {
           p.stats[2 * int64_t(p.rows) + row] = st.x;
           p.stats[3 * int64_t(p.rows) + row] = st.y;
@@ -505,26 +507,26 @@ struct JoinBwd {
   float alpha, inverse;
 };
 
-template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
+template <typename T, int NT, int NV, int FORM, bool BRANCH, bool PACKED>
 struct BwdTiles {
-  using C = Tile<T, NT, NV, VEC>;
-  using K = std::conditional_t<PACKED, PackedTile<T, NT, NV, VEC>, C>;
+  using C = Tile<T, NT, NV, FORM>;
+  using K = std::conditional_t<PACKED, PackedTile<T, NT, NV, FORM>, C>;
   static __host__ __device__ constexpr int bytes(int cols) { return 2 * C::bytes(cols) + (BRANCH ? 2 : 1) * K::bytes(cols); }
 };
 
 // A row takes two CTA-wide reductions (one without a branch), the second one of
 // values that the first decides.  The column sums stay in registers: 64 of them for
 // sixteen columns a thread, which is what limits an SM to 512 threads.
-template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED, int STAGES>
+template <typename T, int NT, int NV, int FORM, bool BRANCH, bool PACKED, int STAGES>
 __global__ void __launch_bounds__(NT, kSmThreads / NT) join_bwd_kernel(JoinBwd p) {
   constexpr int N = NV * 4;
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float2 sh[2][16];
-  using Tiles = BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>;
+  using Tiles = BwdTiles<T, NT, NV, FORM, BRANCH, PACKED>;
   using C = typename Tiles::C;
   using K = typename Tiles::K;
   const int whole = C::bytes(p.cols), kept = K::bytes(p.cols), bytes = Tiles::bytes(p.cols);
-  clear<NT, VEC>(ring, STAGES * bytes, p.cols == NT * NV * 8);
+  clear<NT, FORM>(ring, STAGES * bytes);
   // For this thread's columns, behind the rows: w as stored, and gate * pw in FP32.
   uint4* const weights = reinterpret_cast<uint4*>(ring + STAGES * bytes);
   constexpr int kW = NV * C::kPieces * NT;  // pieces of w
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) join_bwd_kernel(JoinBwd p
   const int which = threadIdx.x & 3;
   const float* stats = which == 0 ? p.mean_u : which == 1 || !BRANCH ? p.rstd_u : which == 2 ? p.mean_y : p.rstd_y;
   float stat = blockIdx.x < p.rows ? stats[blockIdx.x] : 0.f;
-  walk<NT, VEC, STAGES>(
+  walk<NT, FORM, STAGES>(
       p.rows,
       [&](int64_t row, int stage) {
         char* r = ring + stage * bytes;
@@ -782,50 +784,75 @@ int most_ctas(int by_threads, int ring) {
   return 148 * (fit < by_threads ? (fit < 1 ? 1 : fit) : by_threads);
 }
 
-template <typename T, int NT, int NV, bool VEC>
+// The form of a call: 0 for odd widths and unaligned rows, 1 for vectors, 2 for vectors
+// of a width that fills every thread (no bounds to check).
+template <int NT, int NV>
+int form_of(bool vec, int cols) {
+  return !vec ? 0 : cols == NT * NV * 8 ? 2 : 1;
+}
+
+template <typename T, int NT, int NV, int FORM>
 int fwd_launch(const JoinFwd& p, cudaStream_t s) {
-  const int smem = kFwdStages * 2 * Tile<T, NT, NV, VEC>::bytes(p.cols);
+  const int smem = kFwdStages * 2 * Tile<T, NT, NV, FORM>::bytes(p.cols);
   if (smem > kMaxRing) return -1;
-  if (const int r = opt_in<join_fwd_kernel<T, NT, NV, VEC, kFwdStages>>(smem)) return r;
-  join_fwd_kernel<T, NT, NV, VEC, kFwdStages><<<unsigned(std::min(p.rows, most_ctas(kSmThreads / NT, smem))), NT, smem, s>>>(p);
+  if (const int r = opt_in<join_fwd_kernel<T, NT, NV, FORM, kFwdStages>>(smem)) return r;
+  const int ctas = std::min(p.rows, most_ctas(kSmThreads / NT, smem));
+  join_fwd_kernel<T, NT, NV, FORM, kFwdStages><<<unsigned(ctas), NT, smem, s>>>(p);
   return int(cudaGetLastError());
 }
-template <typename T, bool VEC>
-int fwd_pick(const JoinFwd& p, cudaStream_t s) {
-  if (p.cols <= 256) return fwd_launch<T, 32, 1, VEC>(p, s);
-  if (p.cols <= 1024) return fwd_launch<T, 128, 1, VEC>(p, s);
+template <typename T, int NT, int NV>
+int fwd_form(const JoinFwd& p, bool vec, cudaStream_t s) {
+  switch (form_of<NT, NV>(vec, p.cols)) {
+    case 2: return fwd_launch<T, NT, NV, 2>(p, s);
+    case 1: return fwd_launch<T, NT, NV, 1>(p, s);
+    default: return fwd_launch<T, NT, NV, 0>(p, s);
+  }
+}
+template <typename T>
+int fwd_pick(const JoinFwd& p, bool vec, cudaStream_t s) {
+  if (p.cols <= 256) return fwd_form<T, 32, 1>(p, vec, s);
+  if (p.cols <= 1024) return fwd_form<T, 128, 1>(p, vec, s);
   // FP32 rows leave room for half as many CTAs, so they have twice the threads.
   constexpr int kMore = sizeof(T) == 4 ? 2 : 1;
-  if (p.cols <= 2048) return fwd_launch<T, 128 * kMore, 2 / kMore, VEC>(p, s);
-  if (p.cols <= 4096) return fwd_launch<T, 128 * kMore, 4 / kMore, VEC>(p, s);
-  return fwd_launch<T, 256 * kMore, 4 / kMore, VEC>(p, s);
+  if (p.cols <= 2048) return fwd_form<T, 128 * kMore, 2 / kMore>(p, vec, s);
+  if (p.cols <= 4096) return fwd_form<T, 128 * kMore, 4 / kMore>(p, vec, s);
+  return fwd_form<T, 256 * kMore, 4 / kMore>(p, vec, s);
 }
 
 // The gradient's CTAs: as many as fit, but four rows each where that leaves every SM one.
-template <typename T, int NT, int NV, bool VEC, bool BRANCH, bool PACKED>
+template <typename T, int NT, int NV, int FORM, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   // Two rows of the widest FP32 tensors are more than an SM holds.
   constexpr int kRows = sizeof(T) == 4 && NT * NV == 1024 ? 1 : kBwdStages;
-  const int smem = kRows * BwdTiles<T, NT, NV, VEC, BRANCH, PACKED>::bytes(p.cols) + NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
+  const int smem = kRows * BwdTiles<T, NT, NV, FORM, BRANCH, PACKED>::bytes(p.cols) +
+                   NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
   if (smem > kMaxRing) return -1;
-  if (const int r = opt_in<join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows>>(smem)) return r;
+  if (const int r = opt_in<join_bwd_kernel<T, NT, NV, FORM, BRANCH, PACKED, kRows>>(smem)) return r;
   f.parts = std::min(std::min(p.rows, most_ctas(kSmThreads / NT, smem)), std::max(p.rows / 4, 148));
-  join_bwd_kernel<T, NT, NV, VEC, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
+  join_bwd_kernel<T, NT, NV, FORM, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
   if (const int r = int(cudaGetLastError())) return r;
   constexpr bool kWide = NT * NV * 8 > 2048;
   constexpr int kCols = kWide ? 32 : BRANCH ? 8 : 16;
   join_finish_kernel<T, BRANCH, kWide><<<unsigned((p.cols + kCols - 1) / kCols), 1024, 0, s>>>(f);
   return int(cudaGetLastError());
 }
-template <typename T, bool VEC, bool BRANCH, bool PACKED>
-int bwd_pick(const JoinBwd& p, const JoinFinish& f, cudaStream_t s) {
-  if (p.cols <= 256) return bwd_launch<T, 32, 1, VEC, BRANCH, PACKED>(p, f, s);
-  if (p.cols <= 1024) return bwd_launch<T, 128, 1, VEC, BRANCH, PACKED>(p, f, s);
+template <typename T, int NT, int NV, bool BRANCH, bool PACKED>
+int bwd_form(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
+  switch (form_of<NT, NV>(vec, p.cols)) {
+    case 2: return bwd_launch<T, NT, NV, 2, BRANCH, PACKED>(p, f, s);
+    case 1: return bwd_launch<T, NT, NV, 1, BRANCH, PACKED>(p, f, s);
+    default: return bwd_launch<T, NT, NV, 0, BRANCH, PACKED>(p, f, s);
+  }
+}
+template <typename T, bool BRANCH, bool PACKED>
+int bwd_pick(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
+  if (p.cols <= 256) return bwd_form<T, 32, 1, BRANCH, PACKED>(p, f, vec, s);
+  if (p.cols <= 1024) return bwd_form<T, 128, 1, BRANCH, PACKED>(p, f, vec, s);
   // FP32 rows leave room for half as many CTAs, so they have twice the threads.
   constexpr bool kLong = sizeof(T) == 4 && !PACKED;
-  if (p.cols <= 2048) return bwd_launch<T, kLong ? 256 : 128, kLong ? 1 : 2, VEC, BRANCH, PACKED>(p, f, s);
-  if (p.cols <= 4096) return bwd_launch<T, kLong ? 512 : 256, kLong ? 1 : 2, VEC, BRANCH, PACKED>(p, f, s);
-  return bwd_launch<T, 512, 2, VEC, BRANCH, PACKED>(p, f, s);
+  if (p.cols <= 2048) return bwd_form<T, kLong ? 256 : 128, kLong ? 1 : 2, BRANCH, PACKED>(p, f, vec, s);
+  if (p.cols <= 4096) return bwd_form<T, kLong ? 512 : 256, kLong ? 1 : 2, BRANCH, PACKED>(p, f, vec, s);
+  return bwd_form<T, 512, 2, BRANCH, PACKED>(p, f, vec, s);
 }
 }  // namespace
 
@@ -846,8 +873,8 @@ int join_fwd(const void* x, int64_t ld_x, const void* y, int64_t ld_y, int type,
   const bool vec = cols % 8 == 0 && ld_x * size % 16 == 0 && ld_y * size % 16 == 0 && ld_h * size % 16 == 0 &&
                    aligned16(x) && aligned16(y) && aligned16(pw) && aligned16(pb) && aligned16(gate) && aligned16(w) &&
                    aligned16(b) && aligned16(u) && aligned16(h);
-  if (type == kTypeBF16) return vec ? fwd_pick<__nv_bfloat16, true>(p, s) : fwd_pick<__nv_bfloat16, false>(p, s);
-  if (type == kTypeFP32) return vec ? fwd_pick<float, true>(p, s) : fwd_pick<float, false>(p, s);
+  if (type == kTypeBF16) return fwd_pick<__nv_bfloat16>(p, vec, s);
+  if (type == kTypeFP32) return fwd_pick<float>(p, vec, s);
   return -1;
 }
 
@@ -867,9 +894,8 @@ int join_bwd(const JoinBwdCall& c, cudaStream_t s) {
                    (c.packed || (fine(c.u, c.ld_u) && fine(c.y, c.ld_y)));
   auto pick = [&](auto zero) {
     using T = decltype(zero);
-    if (!branch) return vec ? bwd_pick<T, true, false, true>(p, f, s) : bwd_pick<T, false, false, true>(p, f, s);
-    if (c.packed) return vec ? bwd_pick<T, true, true, true>(p, f, s) : bwd_pick<T, false, true, true>(p, f, s);
-    return vec ? bwd_pick<T, true, true, false>(p, f, s) : bwd_pick<T, false, true, false>(p, f, s);
+    if (!branch) return bwd_pick<T, false, true>(p, f, vec, s);
+    return c.packed ? bwd_pick<T, true, true>(p, f, vec, s) : bwd_pick<T, true, false>(p, f, vec, s);
   };
   if (c.type == kTypeBF16) return pick(__nv_bfloat16());
   if (c.type == kTypeFP32) return pick(float());
