@@ -54,9 +54,9 @@ __device__ __forceinline__ float cta_sum(float v, float* sh) {
     __syncthreads();
     v = 0.f;
 #pragma unroll
-    for (int w = 0; w < NT / 128; ++w) {
-      const float4 q = reinterpret_cast<const float4*>(sh)[w];
-      v += (q.x + q.y) + (q.z + q.w);
+    for (int w = 0; w < NT / 64; ++w) {
+      const float2 q = reinterpret_cast<const float2*>(sh)[w];
+      v += q.x + q.y;
     }
   }
   return v;
@@ -810,11 +810,14 @@ int fwd_form(const JoinFwd& p, bool vec, cudaStream_t s) {
 }
 template <typename T>
 int fwd_pick(const JoinFwd& p, bool vec, cudaStream_t s) {
+  // As few threads a row as registers allow: what a row costs beside its columns, the
+  // reductions, grows with its warps.
   if (p.cols <= 256) return fwd_form<T, 32, 1>(p, vec, s);
-  if (p.cols <= 1024) return fwd_form<T, 128, 1>(p, vec, s);
+  if (p.cols <= 512) return fwd_form<T, 32, 2>(p, vec, s);
   // FP32 rows leave room for half as many CTAs, so they have twice the threads.
   constexpr int kMore = sizeof(T) == 4 ? 2 : 1;
-  if (p.cols <= 2048) return fwd_form<T, 128 * kMore, 2 / kMore>(p, vec, s);
+  if (p.cols <= 1024) return fwd_form<T, 32 * kMore, 4 / kMore>(p, vec, s);
+  if (p.cols <= 2048) return fwd_form<T, 64 * kMore, 4 / kMore>(p, vec, s);
   if (p.cols <= 4096) return fwd_form<T, 128 * kMore, 4 / kMore>(p, vec, s);
   return fwd_form<T, 256 * kMore, 4 / kMore>(p, vec, s);
 }
@@ -847,9 +850,10 @@ int bwd_form(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
 template <typename T, bool BRANCH, bool PACKED>
 int bwd_pick(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
   if (p.cols <= 256) return bwd_form<T, 32, 1, BRANCH, PACKED>(p, f, vec, s);
-  if (p.cols <= 1024) return bwd_form<T, 128, 1, BRANCH, PACKED>(p, f, vec, s);
   // FP32 rows leave room for half as many CTAs, so they have twice the threads.
   constexpr bool kLong = sizeof(T) == 4 && !PACKED;
+  if (p.cols <= 512) return bwd_form<T, 32, 2, BRANCH, PACKED>(p, f, vec, s);
+  if (p.cols <= 1024) return bwd_form<T, kLong ? 128 : 64, kLong ? 1 : 2, BRANCH, PACKED>(p, f, vec, s);
   if (p.cols <= 2048) return bwd_form<T, kLong ? 256 : 128, kLong ? 1 : 2, BRANCH, PACKED>(p, f, vec, s);
   if (p.cols <= 4096) return bwd_form<T, kLong ? 512 : 256, kLong ? 1 : 2, BRANCH, PACKED>(p, f, vec, s);
   return bwd_form<T, 512, 2, BRANCH, PACKED>(p, f, vec, s);
@@ -859,7 +863,7 @@ int bwd_pick(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
 int64_t join_max_cols() { return kJoinMaxCols; }
 int join_bwd_parts(int64_t rows, int64_t cols) {
   // The most that any form launches at this width (threads alone).
-  const int nt = cols <= 256 ? 32 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
+  const int nt = cols <= 512 ? 32 : cols <= 1024 ? 64 : cols <= 2048 ? 128 : cols <= 4096 ? 256 : 512;
   return int(std::min<int64_t>(rows, 148 * (kSmThreads / nt)));
 }
 
