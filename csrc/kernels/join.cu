@@ -822,7 +822,9 @@ int fwd_pick(const JoinFwd& p, bool vec, cudaStream_t s) {
   return fwd_form<T, 256 * kMore, 4 / kMore>(p, vec, s);
 }
 
-// The gradient's CTAs: as many as fit, but four rows each where that leaves every SM one.
+// The gradient's CTAs: as many as fit, but some rows each where that leaves every SM one:
+// every CTA's column sums are written and read once. 777 x 2048: four rows and two cost the
+// same; odd widths, whose rows take longer, 20 us with four and 16 with two at 777 x 2050.
 template <typename T, int NT, int NV, int FORM, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   // Two rows of the widest FP32 tensors are more than an SM holds.
@@ -831,7 +833,7 @@ int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
                    NT * NV * (8 * int(sizeof(T)) + (BRANCH ? 32 : 0));
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_bwd_kernel<T, NT, NV, FORM, BRANCH, PACKED, kRows>>(smem)) return r;
-  f.parts = std::min(std::min(p.rows, most_ctas(kSmThreads / NT, smem)), std::max(p.rows / 4, 148));
+  f.parts = std::min(std::min(p.rows, most_ctas(kSmThreads / NT, smem)), std::max(p.rows / (FORM ? 4 : 2), 148));
   join_bwd_kernel<T, NT, NV, FORM, BRANCH, PACKED, kRows><<<unsigned(f.parts), NT, smem, s>>>(p);
   if (const int r = int(cudaGetLastError())) return r;
   constexpr bool kWide = NT * NV * 8 > 2048;

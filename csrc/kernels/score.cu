@@ -694,12 +694,20 @@ __global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, in
   const bool empty = m == -INFINITY;
   const int64_t local = target - start;
   const unsigned at = local >= 0 && local < vocab ? unsigned(local) : 0xffffffffu;
+  // -p (a + b (l + H)) as p (c0 + c1 l), l = ln p; nothing in a row that the mask emptied.
+  const float c1 = empty ? 0.f : -b, c0 = empty ? 0.f : -a - b * H;
   auto gradient = [&](float z, unsigned i) {
     const float l = fmaxf((z - m) - ln_s, kLowest);
-    const float p = fast_exp2(l * kLog2e);
-    float g = -p * (a + b * (l + H));
-    if (i == at) g += a;
-    return empty ? 0.f : g;
+    const float g = fast_exp2(l * kLog2e) * fmaf(c1, l, c0);
+    return i == at && !empty ? g + a : g;
+  };
+  const Two minus_m = two(-m, -m), minus_ln_s = two(-ln_s, -ln_s), scale = two(kLog2e, kLog2e);
+  const Two c0s = two(c0, c0), c1s = two(c1, c1);
+  auto gradients = [&](Two z) {
+    const float2 d = both(two_add(two_add(z, minus_m), minus_ln_s));
+    const Two l = two(fmaxf(d.x, kLowest), fmaxf(d.y, kLowest));
+    const float2 t = both(two_mul(l, scale));
+    return two_mul(two(fast_exp2(t.x), fast_exp2(t.y)), two_fma(c1s, l, c0s));
   };
   const T* x = logits + int64_t(row) * ld;
   T* y = out + int64_t(row) * ld_out;
@@ -719,7 +727,16 @@ __global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, in
       vec[i].get(v);
       T* h = reinterpret_cast<T*>(&vec[i].raw);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) h[e] = from_float<T>(gradient(v[e], c + e));
+      for (int e = 0; e < kN; e += 2) {
+        const float2 g = both(gradients(two(v[e], v[e + 1])));
+        h[e] = from_float<T>(g.x);
+        h[e + 1] = from_float<T>(g.y);
+      }
+      if (at - c < unsigned(kN)) {  // the given token's own vector
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+          if (c + e == at) h[e] = from_float<T>(gradient(v[e], at));
+      }
       *reinterpret_cast<uint4*>(y + c) = vec[i].raw;
     }
     if (block == 0 && threadIdx.x < part.head + part.tail) {
