@@ -696,6 +696,7 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) join_bwd_kernel(JoinBwd p
           }
         }
       });
+  cudaTriggerProgrammaticLaunchCompletion();
   float* out = p.sums + int64_t(blockIdx.x) * (BRANCH ? 4 : 2) * p.cols;
 #pragma unroll
   for (int g = 0; g < NV; ++g) {
@@ -727,6 +728,7 @@ __global__ void __launch_bounds__(1024) join_finish_kernel(JoinFinish p) {
   const int col = blockIdx.x * kCols + lane % kCols;
   const bool has = col < p.cols;
   float s[kEach] = {};
+  cudaGridDependencySynchronize();
   if (has) {
     const float* from = p.sums + int64_t(lane / kCols) * p.cols + col;
 #pragma unroll 4
@@ -838,8 +840,17 @@ int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   if (const int r = int(cudaGetLastError())) return r;
   constexpr bool kWide = NT * NV * 8 > 2048;
   constexpr int kCols = kWide ? 32 : BRANCH ? 8 : 16;
-  join_finish_kernel<T, BRANCH, kWide><<<unsigned((p.cols + kCols - 1) / kCols), 1024, 0, s>>>(f);
-  return int(cudaGetLastError());
+  // Launched while the rows' last CTAs run; it waits for them itself.
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned((p.cols + kCols - 1) / kCols));
+  config.blockDim = dim3(1024);
+  config.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return int(cudaLaunchKernelEx(&config, join_finish_kernel<T, BRANCH, kWide>, f));
 }
 template <typename T, int NT, int NV, bool BRANCH, bool PACKED>
 int bwd_form(const JoinBwd& p, const JoinFinish& f, bool vec, cudaStream_t s) {
