@@ -127,8 +127,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
                    world: int = 1):
     """Return (TokenScores, ScoreState) of logits [M, V/world] (this rank's shard).
 
-    A negative target is not scored (log probability 0, no gradient); one at or
-    above the vocabulary's end gives NaN.  A logit of -inf is a token that cannot
+    A negative target is not scored (log probability 0, which passes no gradient on;
+    the entropy is the row's all the same); one at or above the vocabulary's end
+    gives NaN.  A logit of -inf is a token that cannot
     occur; a row of nothing else has log probability -inf, entropy 0 and no
     gradient.  A NaN or +inf makes its row's numbers NaN.  `top_k` is at most 32
     and at most the shard's vocabulary.

@@ -498,3 +498,32 @@ def test_outputs_may_take_the_place_of_inputs():
         work = du.clone()
         got = norm.layer_norm_bwd_packed(dh, p, j["w"], stats[2], stats[3], dres=work, out=work)
         assert all(torch.equal(p, q) for p, q in zip(got[:3], want[:3]))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("H", [256, 512, 1024, 2048, 4096, 8192])
+def test_widths_that_fill_the_threads_over_many_rows(H, dtype):
+    """Several rows per CTA, one after another through the same shared memory."""
+    actpack, _, norm = ops()
+    rows = 1501
+    j = joint(60 + H, rows, H, dtype)
+    got = norm.block_join_fwd(*j.values(), 1e-5, residual_scale=0.9)
+    check_joint(got, j, 1e-5, 0.9, dtype)
+    x_out, _, stats = got
+    dh, du = randn(61, rows, H, to=dtype), randn(62, rows, H, to=dtype)
+    rest = (stats, j["pw"], j["pb"], j["gate"], j["w"])
+    want, size = ref.join_grad(dh, du, x_out, j["y"], *rest, 0.9)
+    check_grads(norm.block_join_bwd(dh, du, x_out, j["y"], *rest, residual_scale=0.9), want, size, rows, dtype)
+    del want, size
+    pu, py = actpack.pack(x_out), actpack.pack(j["y"])
+    u8, y8 = ref.kept(x_out), ref.kept(j["y"])
+    want, size = ref.join_grad(dh, du, u8, y8, *rest, 0.9)
+    g = norm.block_join_bwd(dh, du, pu, py, *rest, residual_scale=0.9, pre_bias=j["b"])
+    check_grads(g, want, size, rows, dtype)
+    dx, dw, db, y = norm.layer_norm_bwd_packed(dh, pu, j["w"], stats[2], stats[3], dres=du, bias=j["b"])
+    assert torch.equal(y, g.h)
+    one = torch.ones(H, device="cuda")
+    lw, ls = ref.join_grad(dh, du, u8, y8, stats, one, one, one, j["w"], 1.0)
+    check_grads((dx, dx), (lw[0], lw[0]), (ls[0], ls[0]), rows, dtype)
+    for a, k in ((dw, 5), (db, 6)):
+        ref.close(a, lw[k], ref.rounded(lw[k], dtype) + (64 + rows / 148 + 148 / 8 + 8) * ref.U * ls[k])
