@@ -2,6 +2,8 @@
 // current CUDA stream is used; every launch failure raises.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <ATen/ops/as_strided_native.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "kernels_api.h"
@@ -430,7 +432,17 @@ void join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, const a
 
 // The operators' public forms: outputs are allocated here, so that a call costs one
 // crossing from Python.  Arguments are checked by the functions above.
-at::Tensor rows_like(const at::Tensor& t) { return at::empty({t.size(0), t.size(1)}, t.options()); }
+// Outputs and their parts are made without the dispatcher, which would cost more than a
+// small kernel: they are plain tensors on `like`'s device.
+at::Tensor fresh(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+at::Tensor rows_like(const at::Tensor& t) { return fresh(t, {t.size(0), t.size(1)}, t.scalar_type()); }
+at::Tensor part(const at::Tensor& t, at::IntArrayRef sizes, int64_t offset) {
+  const int64_t inner = sizes.size() == 2 ? std::max<int64_t>(sizes[1], 1) : 1;
+  if (sizes.size() == 2) return at::native::as_strided_tensorimpl(t, sizes, {inner, 1}, offset);
+  return at::native::as_strided_tensorimpl(t, sizes, {1}, offset);
+}
 void need_matrix(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 2, name, " must be a matrix on CUDA");
 }
@@ -443,12 +455,11 @@ Tensors token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int6
   need_matrix(logits, "logits");
   TORCH_CHECK(top_k >= 0 && top_k <= 32, "top_k is out of range");
   const int64_t rows = logits.size(0);
-  at::Tensor out = at::empty({rows * (5 + top_k)}, logits.options().dtype(at::kFloat));
-  at::Tensor ids = at::empty({rows, top_k}, logits.options().dtype(at::kLong));
+  at::Tensor out = fresh(logits, {rows * (5 + top_k)}, at::kFloat);
+  at::Tensor ids = fresh(logits, {rows, top_k}, at::kLong);
   if (rows) score_fwd(logits, targets.contiguous(), 0, logits.size(1), top_k, out, ids, c10::nullopt);
-  return {out.as_strided({rows}, {1}, 0), out.as_strided({rows}, {1}, rows),
-          out.as_strided({rows, top_k}, {std::max<int64_t>(top_k, 1), 1}, 5 * rows), ids,
-          out.as_strided({3, rows}, {std::max<int64_t>(rows, 1), 1}, 2 * rows)};
+  return {part(out, {rows}, 0), part(out, {rows}, rows), part(out, {rows, top_k}, 5 * rows), ids,
+          part(out, {3, rows}, 2 * rows)};
 }
 at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& targets, int64_t start,
                                    int64_t vocab_total, const at::Tensor& state, const at::Tensor& dlogprob,
@@ -469,14 +480,16 @@ at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& t
 }
 at::Tensor pack(const at::Tensor& x) {
   need_matrix(x, "x");
-  at::Tensor data = at::empty({x.size(0), k::act_pack_row_bytes(x.size(1))}, x.options().dtype(at::kByte));
+  at::Tensor data = fresh(x, {x.size(0), k::act_pack_row_bytes(x.size(1))}, at::kByte);
   if (x.size(0)) act_pack(x, data);
   return data;
 }
 Tensors unpack(const at::Tensor& data, int64_t cols, bool fp32, bool gelu) {
-  at::Tensor out = at::empty({data.size(0), cols}, data.options().dtype(fp32 ? at::kFloat : at::kBFloat16));
+  need_matrix(data, "data");
+  const at::ScalarType type = fp32 ? at::kFloat : at::kBFloat16;
+  at::Tensor out = fresh(data, {data.size(0), cols}, type);
   c10::optional<at::Tensor> act;
-  if (gelu) act = at::empty_like(out);
+  if (gelu) act = fresh(data, {data.size(0), cols}, type);
   if (out.numel()) act_unpack(data, out, act);
   return {out, act};
 }
@@ -487,7 +500,7 @@ Tensors block_join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tenso
   need_own_rows(out, "out");
   at::Tensor u = rows_like(x);
   at::Tensor h = out ? *out : rows_like(x);
-  at::Tensor stats = at::empty({4, x.size(0)}, x.options().dtype(at::kFloat));
+  at::Tensor stats = fresh(x, {4, x.size(0)}, at::kFloat);
   if (x.size(0)) join_fwd(x, y, pw, pb, gate, w, b, u, h, stats, alpha, eps);
   return {u, h, stats};
 }
@@ -496,13 +509,13 @@ struct Spare {  // gradients of the parameters, and a workspace that is large en
   Spare(const at::Tensor& dh, bool branch, const c10::optional<at::Tensor>& given) {
     const int64_t rows = dh.size(0), cols = dh.size(1);
     TORCH_CHECK(cols > 0 && cols <= k::join_max_cols(), "the hidden size is out of range");
-    grads = at::empty({branch ? 5 : 2, cols}, dh.options());
+    grads = fresh(dh, {branch ? 5 : 2, cols}, dh.scalar_type());
     if (!rows) {
       grads.zero_();
       return;
     }
     const int64_t size = join_bwd_workspace(rows, cols, branch);
-    workspace = given && given->numel() >= size ? *given : at::empty({size}, dh.options().dtype(at::kFloat));
+    workspace = given && given->numel() >= size ? *given : fresh(dh, {size}, at::kFloat);
   }
 };
 // (dx, dy, dpost_weight, dpost_bias, dgate, dpre_weight, dpre_bias, h)
@@ -526,7 +539,7 @@ Tensors block_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du
                  spare.grads, spare.workspace, alpha);
   }
   const int64_t cols = dh.size(1);
-  auto grad = [&](int i) { return spare.grads.as_strided({cols}, {1}, i * cols); };
+  auto grad = [&](int i) { return part(spare.grads, {cols}, i * cols); };
   return {dx, dy, grad(2), grad(3), grad(4), grad(0), grad(1), h};
 }
 // (dx, dweight, dbias, y)
@@ -546,7 +559,8 @@ Tensors layer_norm_bwd_packed(const at::Tensor& dy, const c10::optional<at::Tens
   if (dy.size(0))
     run_join_bwd(dy, dres, x, none, RowStats{mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr}, none,
                  none, none, w, b, dx, none, y, spare.grads, spare.workspace, 1.0);
-  return {dx, spare.grads.select(0, 0), spare.grads.select(0, 1), y};
+  const int64_t cols = dy.size(1);
+  return {dx, part(spare.grads, {cols}, 0), part(spare.grads, {cols}, cols), y};
 }
 }  // namespace
 
