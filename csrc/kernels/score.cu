@@ -552,13 +552,18 @@ __global__ void __launch_bounds__(NT, kSmThreads / NT) score_kernel(const T* log
       for (int i = 0; i < kUnroll; ++i) raw[i] = vectors[j + i * NT];
       run.template add<kUnroll>(raw);
     }
-    for (; j < part.vectors; j += NT) {
-      const uint4 raw = vectors[j];
-      run.template add<1>(&raw);
-    }
-    if (unsigned(tid) < part.tail) {
-      run.add_one(to_float(part.x[part.vector_at(part.vectors) + tid]));
-    }
+    // What is left, loaded together as well: one after another these would cost a short
+    // row most of its time.
+    uint4 last[kUnroll - 1];
+#pragma unroll
+    for (int i = 0; i < kUnroll - 1; ++i)
+      if (j + i * NT < part.vectors) last[i] = vectors[j + i * NT];
+    float tail = 0.f;
+    if (unsigned(tid) < part.tail) tail = to_float(part.x[part.vector_at(part.vectors) + tid]);
+#pragma unroll
+    for (int i = 0; i < kUnroll - 1; ++i)
+      if (j + i * NT < part.vectors) run.template add<1>(last + i);
+    if (unsigned(tid) < part.tail) run.add_one(tail);
     const Sums a = run.warp_total();
     own = run.m;
     if (lane == 0) warp_sums[warp] = a;
