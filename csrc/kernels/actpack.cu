@@ -145,31 +145,41 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsig
   }
 }
 
-// Odd widths and unaligned rows: a warp per group, single values, contiguous over the warp.
+// Odd widths and unaligned rows: a warp has four groups, single values, 32 at a time,
+// contiguous over the warp and all on their way at once.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_odd_kernel(const T* x, int64_t ld, unsigned char* data, int cols,
-                                                       unsigned groups, unsigned items) {
+                                                       unsigned segments, unsigned items) {
+  constexpr int kGroups = 4;
   const int lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * 8u + threadIdx.x / 32u;
   if (item >= items) return;
-  const unsigned row = item / groups, group = item - row * groups;
-  const int col = int(group) * kPackGroup + lane;
+  const unsigned row = item / segments, first = (item - row * segments) * kGroups;
+  const int col = int(first) * kPackGroup + lane, groups = int(pack_groups(cols));
   const T* src = x + int64_t(row) * ld;
-  float v[4], amax = 0.f;
+  float v[kGroups * 4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = col + i * 32 < cols ? to_float(src[col + i * 32]) : 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) amax = max_nan(amax, fabsf(v[i]));
-  const unsigned byte = settle<32, 4>(v, amax);
-  const float inverse = inverse_unit(byte);
+  for (int i = 0; i < kGroups * 4; ++i) v[i] = col + i * 32 < cols ? to_float(src[col + i * 32]) : 0.f;
   unsigned char* dst = data + int64_t(row) * pack_row_bytes(cols);
   const int code_bytes = int(pack_code_bytes(cols));
+  unsigned bytes = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i * 32 < code_bytes) dst[col + i * 32] = static_cast<unsigned char>(encode2(v[i], 0.f, inverse) & 0xffu);
+  for (int g = 0; g < kGroups; ++g) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) amax = max_nan(amax, fabsf(v[g * 4 + i]));
+    const unsigned byte = settle<32, 4>(v + g * 4, amax);
+    const float inverse = inverse_unit(byte);
+    bytes |= byte << (8 * g);
+#pragma unroll
+    for (int i = g * 4; i < g * 4 + 4; ++i)
+      if (col + i * 32 < code_bytes) dst[col + i * 32] = static_cast<unsigned char>(encode2(v[i], 0.f, inverse) & 0xffu);
+  }
+  // Exponent bytes, then zeros up to the padding's end.
   unsigned char* units = dst + code_bytes;
-  if (lane == 0) units[group] = static_cast<unsigned char>(byte);
-  if (group == groups - 1 && groups + lane < (groups + 15u) / 16u * 16u) units[groups + lane] = 0;
+  const int mine = int(first) + lane;
+  if (lane < kGroups && mine < groups) units[mine] = static_cast<unsigned char>(bytes >> (8 * lane));
+  if (int(first) + kGroups >= groups && groups + lane < (groups + 15) / 16 * 16) units[groups + lane] = 0;
 }
 
 // GeLU(v) = v * Phi(v) of a kept value.  Kept values have three mantissa bits, so
@@ -321,11 +331,11 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 template <typename T>
 int pack_typed(const void* x, int64_t ld, void* data, int64_t rows, int64_t cols, cudaStream_t s) {
-  const int64_t groups = pack_groups(cols), items = rows * groups;
   const bool vec = cols % 8 == 0 && ld * int64_t(sizeof(T)) % 16 == 0 && aligned16(x);
+  const int64_t pieces = vec ? pack_groups(cols) : (cols + 511) / 512, items = rows * pieces;
   auto launch = [&](auto kernel, int64_t per_cta) {
     kernel<<<unsigned((items + per_cta - 1) / per_cta), 256, 0, s>>>(
-        static_cast<const T*>(x), ld, static_cast<unsigned char*>(data), int(cols), unsigned(groups), unsigned(items));
+        static_cast<const T*>(x), ld, static_cast<unsigned char*>(data), int(cols), unsigned(pieces), unsigned(items));
   };
   vec ? launch(pack_kernel<T>, 32) : launch(pack_odd_kernel<T>, 8);
   return int(cudaGetLastError());

@@ -45,7 +45,11 @@ namespace tn5b {
 namespace kernels {
 namespace {
 constexpr int kMaxRing = 200 * 1024;  // of an SM's 227 KB, for all CTAs on it
-constexpr int kFwdStages = 3, kBwdStages = 2;
+constexpr int kFwdStages = 2, kBwdStages = 2;
+// Threads of all CTAs on an SM, forward: 96 or 80 registers each.  8192 x 4096 BF16: 640
+// threads 47 us, 512 with a third row ahead 55, 768 49; two CTAs of 256 against three at
+// 4096 x 8192: 60 and 50 us.
+__host__ __device__ constexpr int fwd_threads(int nt) { return nt <= 128 ? 640 : 768; }
 constexpr int kSmThreads = 512;  // of all CTAs on an SM, at 128 registers each
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -441,7 +445,7 @@ __device__ __forceinline__ float2 row_stats(const Two* v, const JoinFwd& p, floa
 }
 
 template <typename T, int NT, int NV, int FORM, int STAGES>
-__global__ void __launch_bounds__(NT, kSmThreads / NT) join_fwd_kernel(JoinFwd p) {
+__global__ void __launch_bounds__(NT, fwd_threads(NT) / NT) join_fwd_kernel(JoinFwd p) {
   extern __shared__ __align__(16) char ring[];
   __shared__ __align__(16) float sh[64];
   using C = Tile<T, NT, NV, FORM>;
@@ -805,7 +809,7 @@ int fwd_launch(const JoinFwd& p, cudaStream_t s) {
   const int smem = kFwdStages * 2 * Tile<T, NT, NV, FORM>::bytes(p.cols);
   if (smem > kMaxRing) return -1;
   if (const int r = opt_in<join_fwd_kernel<T, NT, NV, FORM, kFwdStages>>(smem)) return r;
-  const int ctas = std::min(p.rows, most_ctas(kSmThreads / NT, smem));
+  const int ctas = std::min(p.rows, most_ctas(fwd_threads(NT) / NT, smem));
   join_fwd_kernel<T, NT, NV, FORM, kFwdStages><<<unsigned(ctas), NT, smem, s>>>(p);
   return int(cudaGetLastError());
 }
