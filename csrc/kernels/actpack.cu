@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* x, int64_t ld, unsig
   }
 }
 
-// Odd widths and unaligned rows: a warp has four groups, single values, 32 at a time,
-// contiguous over the warp and all on their way at once.
+// Odd widths and unaligned rows: a warp has four groups, a lane pairs of columns (loaded
+// one by one, their codes stored together), all on their way at once.
 template <typename T>
 __global__ void __launch_bounds__(256) pack_odd_kernel(const T* x, int64_t ld, unsigned char* data, int cols,
                                                        unsigned segments, unsigned items) {
@@ -155,11 +155,14 @@ __global__ void __launch_bounds__(256) pack_odd_kernel(const T* x, int64_t ld, u
   const unsigned item = blockIdx.x * 8u + threadIdx.x / 32u;
   if (item >= items) return;
   const unsigned row = item / segments, first = (item - row * segments) * kGroups;
-  const int col = int(first) * kPackGroup + lane, groups = int(pack_groups(cols));
+  const int col = int(first) * kPackGroup + 2 * lane, groups = int(pack_groups(cols));
   const T* src = x + int64_t(row) * ld;
-  float v[kGroups * 4];
+  float v[kGroups * 4];  // 2 i and 2 i + 1: columns col + 64 i and the next
 #pragma unroll
-  for (int i = 0; i < kGroups * 4; ++i) v[i] = col + i * 32 < cols ? to_float(src[col + i * 32]) : 0.f;
+  for (int i = 0; i < kGroups * 4; ++i) {
+    const int c = col + i / 2 * 64 + (i & 1);
+    v[i] = c < cols ? to_float(src[c]) : 0.f;
+  }
   unsigned char* dst = data + int64_t(row) * pack_row_bytes(cols);
   const int code_bytes = int(pack_code_bytes(cols));
   unsigned bytes = 0;
@@ -172,8 +175,9 @@ __global__ void __launch_bounds__(256) pack_odd_kernel(const T* x, int64_t ld, u
     const float inverse = inverse_unit(byte);
     bytes |= byte << (8 * g);
 #pragma unroll
-    for (int i = g * 4; i < g * 4 + 4; ++i)
-      if (col + i * 32 < code_bytes) dst[col + i * 32] = static_cast<unsigned char>(encode2(v[i], 0.f, inverse) & 0xffu);
+    for (int i = g * 2; i < g * 2 + 2; ++i)
+      if (col + i * 64 < code_bytes)
+        *reinterpret_cast<unsigned short*>(dst + col + i * 64) = encode2(v[2 * i], v[2 * i + 1], inverse);
   }
   // Exponent bytes, then zeros up to the padding's end.
   unsigned char* units = dst + code_bytes;
