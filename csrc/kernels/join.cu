@@ -19,8 +19,8 @@
 // the CTAs in order, without atomics.
 //
 // Both directions are persistent: a CTA takes the rows row, row + grid, .. and has
-// the next ones (two forward, one backward) on their way into shared memory (cp.async)
-// while it works on one, so loads are in flight all the time and no register holds them.
+// the next one on its way into shared memory (cp.async) while it works on one, so
+// loads are in flight all the time and no register holds them.
 //   Vector form (width a multiple of 8, rows on 16-byte boundaries): a thread has
 // pieces of 16 bytes and copies what it will read itself, so it waits for its own
 // copies alone.
@@ -28,12 +28,12 @@
 // row, and threads read single values at the row's offset, columns a CTA's width
 // apart: one barrier more a row.
 //
-// B200, 8192 x 4096 BF16: forward 54 us (5.0 TB/s), gradient 71 us and 6 us for the
+// B200, 8192 x 4096 BF16: forward 48 us (5.6 TB/s), gradient 71 us and 6 us for the
 // column sums (5.3 TB/s), LayerNorm's gradient from 8 bits 63 us (4.8 TB/s).  What
 // bounds them is the time that a row's reductions and its few warps take (issue slots
 // 40-55 %, shared-memory pipe 48-62 % busy); more rows at once would need registers
 // (the column sums) or shared memory that an SM has not.  4095 columns, one by one:
-// 107 and 124 us.
+// 96 and 130 us.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -50,7 +50,7 @@ constexpr int kFwdStages = 2, kBwdStages = 2;
 // threads 47 us, 512 with a third row ahead 55, 768 49; two CTAs of 256 against three at
 // 4096 x 8192: 60 and 50 us.
 __host__ __device__ constexpr int fwd_threads(int nt) { return nt <= 128 ? 640 : 768; }
-constexpr int kSmThreads = 512;  // of all CTAs on an SM, at 128 registers each
+constexpr int kSmThreads = 512;  // the same for the gradient, at 128 registers each
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

@@ -17,9 +17,9 @@
 // Ranks of a vocabulary-parallel group exchange one record a row (m, s, u, z_t
 // and their own alternatives) and merge them in rank order.
 //
-// B200, 8192 BF16 rows of 50304: 129 us without alternatives (6.4 TB/s, the copy's
+// B200, 8192 BF16 rows of 50304: 128 us without alternatives (6.4 TB/s, the copy's
 // rate; the exponentials keep the special-function units 71-76 % busy, which is what
-// bounds it next), 150 us with 8 and 181 us with 32 of them (the second look and the
+// bounds it next), 149 us with 8 and 179 us with 32 of them (the second look and the
 // sorts, between barriers).  Inputs that are not in any cache add 11 us.  Splitting a
 // row over more threads or CTAs costs more than it gives where rows are many.
 // Gradient of 2048 rows: 64 us (6.5 TB/s).
@@ -793,7 +793,7 @@ int score_threads(const void* logits, int64_t ld, unsigned vocab, const int64_t*
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
-  // A row is split over a cluster while the rows alone leave SMs idle (1 row of 50304: 9.8 us
+  // A row is split over a cluster while the rows alone leave SMs idle (1 row of 50304: 9.5 us
   // on four CTAs, 11.6 us on one; with more rows than SMs the split only costs).
   unsigned C = 1;
   while (C < 4 && int64_t(o.rows) * C * 2 <= 148 && vocab / (2 * C) >= 4096) C *= 2;
