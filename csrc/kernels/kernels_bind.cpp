@@ -307,6 +307,7 @@ void need_packed(const at::Tensor& data, const at::Tensor& like, int64_t rows, i
   TORCH_CHECK(data.scalar_type() == at::kByte && data.dim() == 2 && data.is_contiguous() && data.size(0) == rows &&
                   data.size(1) == k::act_pack_row_bytes(cols),
               name, " is not the packed form of ", shape_text(rows, cols));
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, name, " must start on a 16-byte boundary");
 }
 void act_pack(const at::Tensor& x, at::Tensor& data) {
   const int type = type_code(x, false, "x");

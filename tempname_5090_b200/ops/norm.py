@@ -152,6 +152,11 @@ def _check_kept(name, t, like, shape):
         _check_matrix(name, t, like, shape)
 
 
+def _check_kept_width(p, like):
+    if p.cols != like.shape[-1]:
+        raise ValueError(f"packed rows of {p.cols} columns where {like.shape[-1]} are needed")
+
+
 def block_join_fwd(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, eps, residual_scale=1.0, out=None):
     """Returns (x_out, h, stats) for the residual stream x and a branch's output y, [rows, H]:
 
@@ -227,6 +232,11 @@ def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pr
             kept = isinstance(x_out, Packed8)
             if kept != isinstance(y, Packed8):
                 raise ValueError("x_out and y are kept in the same form")
+            if kept:  # rows of another width may take as many bytes
+                _check_kept_width(x_out, dh)
+                _check_kept_width(y, dh)
+            elif x_out.dtype == torch.uint8:
+                raise ValueError("packed rows are given as a Packed8")
             grads = lib().block_join_bwd(dh, dx_out, x_out.data if kept else x_out, y.data if kept else y, stats,
                                          post_weight, post_bias, gate, pre_weight, pre_bias, out, workspace,
                                          residual_scale)
@@ -289,6 +299,7 @@ def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, works
         if not isinstance(x, Packed8):
             raise ValueError("x must be a Packed8")
         try:
+            _check_kept_width(x, dy)
             dx, dw, db, y = lib().layer_norm_bwd_packed(dy, dres, x.data, mean, rstd, weight, bias, out, workspace)
         except (RuntimeError, TypeError):
             _check_packed_norm(dy, x, weight, mean, rstd, dres, bias, out)

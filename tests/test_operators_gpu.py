@@ -527,3 +527,26 @@ def test_widths_that_fill_the_threads_over_many_rows(H, dtype):
     check_grads((dx, dx), (lw[0], lw[0]), (ls[0], ls[0]), rows, dtype)
     for a, k in ((dw, 5), (db, 6)):
         ref.close(a, lw[k], ref.rounded(lw[k], dtype) + (64 + rows / 148 + 148 / 8 + 8) * ref.U * ls[k])
+
+
+def test_refusals_of_other_packed_rows():
+    """Packed rows of another width (250 and 256 columns take as many bytes), raw bytes in
+    their place, and bytes off the 16-byte boundary that the native entries are given."""
+    actpack, _, norm = ops()
+    rows, H = 4, 256
+    j = joint(80, rows, H, BF16)
+    x_out, _, stats = norm.block_join_fwd(*j.values(), 1e-5)
+    dh = randn(81, rows, H)
+    narrow, wide = actpack.pack(x_out[:, :250]), actpack.pack(x_out)
+    rest = (stats, j["pw"], j["pb"], j["gate"], j["w"])
+    for u, y in ((narrow, wide), (wide, narrow), (wide.data, wide.data)):
+        with pytest.raises(ValueError):
+            norm.block_join_bwd(dh, None, u, y, *rest)
+    with pytest.raises(ValueError):
+        norm.layer_norm_bwd_packed(dh, narrow, j["w"], stats[2], stats[3])
+    from tempname_5090_b200._native import lib
+    off = torch.empty(wide.data.numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(wide.data.shape)
+    for call in (lambda: lib().act_pack(x_out, off), lambda: lib().unpack(off, H, False, False),
+                 lambda: lib().layer_norm_bwd_packed(dh, None, off, stats[2], stats[3], j["w"], None, None, None)):
+        with pytest.raises(RuntimeError):
+            call()
