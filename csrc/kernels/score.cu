@@ -195,19 +195,23 @@ struct Running {
 };
 
 // The same for rows whose largest value lies within +-kPlain, in half the
-// instructions: t = z log2 e - R <= 0 with one fused multiply-add, R = fl(m log2 e) the
+// instructions: t = z log2 e - R with one fused multiply-add, R = fl(m log2 e) the
 // running reference, two elements an instruction (f32x2), the maximum of 16-bit
-// types on packed pairs.  Values below -kFloor (-inf above all) are lifted to it,
-// which leaves 2^t zero and t finite.  R is a function of m, so sums join without
-// further state, and its rounding is taken out once per row (`natural`).
-constexpr float kFloor = 1e30f, kPlain = 1e29f;
+// types on packed pairs.  R is a function of m, so sums join without further state.
+// Its rounding, off = m log2 e - R, stays in every t of a sum and is taken out once per
+// row (`natural`).  off is at most half a unit in R's last place: 1/4 for |m| < 2^22,
+// 1 for the lowest start (2^24), so t <= off <= 1 and no exponential overflows.  A row
+// whose largest value is further out would have an off that ruins its sums (128 at
+// 2^31) and takes `Running`.  Values below -kFloor (-inf above all) are lifted to it:
+// 2^t is zero there in any row that counts, and t finite.
+constexpr float kFloor = 33554432.f, kLow = 16777216.f, kPlain = 4194304.f;  // 2^25, 2^24, 2^22
 template <typename T> struct Packed2;
 template <> struct Packed2<__nv_bfloat16> {
   static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
     const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const unsigned*>(&r);
   }
-  static __device__ __forceinline__ unsigned floor() { return 0xf149f149u; }  // -0.995e30
+  static __device__ __forceinline__ unsigned floor() { return 0xcc00cc00u; }  // -kFloor
   static __device__ __forceinline__ Two floats(unsigned w) {
     return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
@@ -247,10 +251,10 @@ struct Loaded<float> {
     for (int i = 0; i < 2; ++i) z[i] = two(fmaxf(v[2 * i], -kFloor), fmaxf(v[2 * i + 1], -kFloor));
   }
 };
-// Where the running maximum begins: at or above every lifted value, so that t <= 0,
-// and so low that what was counted there vanishes in a row whose largest value is
-// above `plain_low` (FP16's floor is no lower than its lowest number).
-template <typename T> __device__ __forceinline__ float start_low() { return -9.9e29f; }
+// Where the running maximum begins: above every lifted value, and so low that what was
+// counted there vanishes in a row whose largest value is above `plain_low` (FP16's floor
+// is its lowest number, where lifted values count 1 until then).
+template <typename T> __device__ __forceinline__ float start_low() { return -kLow; }
 template <> __device__ __forceinline__ float start_low<__half>() { return -65504.f; }
 template <typename T> __device__ __forceinline__ float plain_low() { return -kPlain; }
 template <> __device__ __forceinline__ float plain_low<__half>() { return -6e4f; }
