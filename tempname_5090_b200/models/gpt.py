@@ -481,10 +481,11 @@ class GPT:
             raise ValueError("weights must be FP32, one for each target")
         logits, trunk = self._logits(tokens, targets, keep=True)
         scores, state = CE.token_logprobs(logits, targets, 0, self.tp.group, self.rank, self.world)
-        scored = (targets >= 0).float()
-        w = scored if weights is None else weights * scored
-        bonus = scored * entropy_bonus
-        loss = -((w * scores.logprob).sum() + (bonus * scores.entropy).sum()).reshape(1) / self.M
+        scored = targets >= 0  # chosen, not multiplied: an ignored position may hold anything
+        w = scored.float() if weights is None else torch.where(scored, weights, 0.0)
+        bonus = scored.float() * entropy_bonus
+        loss = -((w * scores.logprob).sum()
+                 + torch.where(scored, bonus * scores.entropy, 0.0).sum()).reshape(1) / self.M
         scale = -loss_scale / self.M
         CE.token_logprobs_backward(logits, targets, state, w * scale, bonus * scale, out=logits)
         self._backward((tokens, targets, trunk, logits, None), loss_scale)
