@@ -241,6 +241,11 @@ void need_floats(const at::Tensor& t, const at::Tensor& like, int64_t n, const c
   TORCH_CHECK(t.numel() >= n, name, " must hold ", std::to_string(n), " values");
 }
 
+void need_vocabulary(int64_t vocab, int64_t vocab_total, int64_t top_k) {
+  TORCH_CHECK(vocab > 0 && vocab_total <= 0x7fffffff, "the vocabulary must have 1 to 2^31 - 1 ids");
+  TORCH_CHECK(top_k >= 0 && top_k <= 32 && top_k <= vocab, "top_k is out of range");
+}
+// Calls without rows are checked like others; there is nothing to launch for them then.
 void score_fwd(const at::Tensor& logits, const at::Tensor& targets, int64_t start, int64_t vocab_total, int64_t top_k,
                const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& top_ids,
                const c10::optional<at::Tensor>& record) {
@@ -248,6 +253,7 @@ void score_fwd(const at::Tensor& logits, const at::Tensor& targets, int64_t star
   const int type = type_code(logits, true, "logits");
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   need_rows(logits, logits, rows, vocab, "logits");
+  need_vocabulary(vocab, vocab_total, top_k);
   need_like(targets, logits, at::kLong, "targets");
   TORCH_CHECK(targets.dim() == 1 && targets.numel() == rows, "targets must hold one id a row");
   float* f = nullptr;
@@ -266,6 +272,7 @@ void score_fwd(const at::Tensor& logits, const at::Tensor& targets, int64_t star
       ids = top_ids->data_ptr<int64_t>();
     }
   }
+  if (!rows) return;
   const c10::cuda::CUDAGuard g(logits.device());
   ok(k::score_fwd(logits.data_ptr(), type, logits.stride(0), rows, vocab, targets.data_ptr<int64_t>(), start,
                   vocab_total, int(top_k), f, f + rows, f + 2 * rows, f + 5 * rows, ids, rec, cur()), "score_fwd");
@@ -290,11 +297,13 @@ void score_bwd(const at::Tensor& logits, const at::Tensor& targets, int64_t star
   const int64_t rows = logits.size(0), vocab = logits.size(1);
   need_rows(logits, logits, rows, vocab, "logits");
   need_rows(out, logits, rows, vocab, "out");
+  need_vocabulary(vocab, vocab_total, 0);
   need_like(targets, logits, at::kLong, "targets");
   TORCH_CHECK(targets.dim() == 1 && targets.numel() == rows, "targets must hold one id a row");
   need_floats(state, logits, 3 * rows, "state");
   need_floats(dlogprob, logits, rows, "dlogprob");
   if (dentropy) need_floats(*dentropy, logits, rows, "dentropy");
+  if (!rows) return;
   const c10::cuda::CUDAGuard g(logits.device());
   ok(k::score_bwd(logits.data_ptr(), type, logits.stride(0), rows, vocab, targets.data_ptr<int64_t>(), start,
                   vocab_total, state.data_ptr<float>(), dlogprob.data_ptr<float>(),
@@ -312,7 +321,9 @@ void need_packed(const at::Tensor& data, const at::Tensor& like, int64_t rows, i
 void act_pack(const at::Tensor& x, at::Tensor& data) {
   const int type = type_code(x, false, "x");
   need_rows(x, x, x.size(0), x.size(1), "x");
+  TORCH_CHECK(x.size(1) > 0, "x needs at least one column");
   need_packed(data, x, x.size(0), x.size(1), "data");
+  if (!x.size(0)) return;
   const c10::cuda::CUDAGuard g(x.device());
   ok(k::act_pack(x.data_ptr(), type, x.stride(0), data.data_ptr(), x.size(0), x.size(1), cur()), "act_pack");
 }
@@ -325,11 +336,15 @@ void act_unpack(const at::Tensor& data, at::Tensor& out, const c10::optional<at:
     need_like(*act, out, out.scalar_type(), "act");
     TORCH_CHECK(act->sizes() == out.sizes(), "act and out differ in shape");
   }
+  if (!out.numel()) return;
   const c10::cuda::CUDAGuard g(out.device());
   ok(k::act_unpack(data.data_ptr(), out.data_ptr(), act ? act->data_ptr() : nullptr, type, rows, cols, cur()),
      "act_unpack");
 }
 
+void need_width(int64_t cols) {
+  TORCH_CHECK(cols > 0 && cols <= k::join_max_cols(), "the hidden size is out of range");
+}
 void join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tensor& pw, const at::Tensor& pb,
               const at::Tensor& gate, const at::Tensor& w, const at::Tensor& b, at::Tensor& u, at::Tensor& h,
               at::Tensor& stats, double alpha, double eps) {
@@ -341,6 +356,8 @@ void join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tensor& pw, co
   need_vector(pw, x, cols, "post_weight"); need_vector(pb, x, cols, "post_bias"); need_vector(gate, x, cols, "gate");
   need_vector(w, x, cols, "pre_weight"); need_vector(b, x, cols, "pre_bias");
   need_floats(stats, x, 4 * rows, "stats");
+  need_width(cols);
+  if (!rows) return;
   const c10::cuda::CUDAGuard g(x.device());
   ok(k::join_fwd(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), type, pw.data_ptr(), pb.data_ptr(),
                  gate.data_ptr(), w.data_ptr(), b.data_ptr(), u.data_ptr(), h.data_ptr(), h.stride(0),
@@ -398,7 +415,7 @@ void run_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, con
   char* gp = static_cast<char*>(grads.data_ptr());
   c.dw = gp; c.db = gp + step;
   if (branch) {
-    TORCH_CHECK(dy && pw && pb && gate && stats.mean_y && stats.rstd_y, "the branch's tensors go together");
+    TORCH_CHECK(dy && pw && pb && gate && (!rows || (stats.mean_y && stats.rstd_y)), "the branch's tensors go together");
     kept(*y, "y");
     need_rows(*dy, dh, rows, cols, "dy");
     need_vector(*pw, dh, cols, "post_weight"); need_vector(*pb, dh, cols, "post_bias");
@@ -411,6 +428,10 @@ void run_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du, con
   }
   need_floats(workspace, dh, join_bwd_workspace(rows, cols, branch), "workspace");
   c.workspace = workspace.data_ptr<float>();
+  if (!rows) {
+    grads.zero_();
+    return;
+  }
   const c10::cuda::CUDAGuard g(dh.device());
   ok(k::join_bwd(c, cur()), branch ? "block_join_bwd" : "layer_norm_bwd_packed");
 }
@@ -454,11 +475,11 @@ using Tensors = std::vector<c10::optional<at::Tensor>>;
 
 Tensors token_logprobs(const at::Tensor& logits, const at::Tensor& targets, int64_t top_k) {
   need_matrix(logits, "logits");
-  TORCH_CHECK(top_k >= 0 && top_k <= 32, "top_k is out of range");
+  need_vocabulary(logits.size(1), logits.size(1), top_k);
   const int64_t rows = logits.size(0);
   at::Tensor out = fresh(logits, {rows * (5 + top_k)}, at::kFloat);
   at::Tensor ids = fresh(logits, {rows, top_k}, at::kLong);
-  if (rows) score_fwd(logits, targets.contiguous(), 0, logits.size(1), top_k, out, ids, c10::nullopt);
+  score_fwd(logits, targets.contiguous(), 0, logits.size(1), top_k, out, ids, c10::nullopt);
   return {part(out, {rows}, 0), part(out, {rows}, rows), part(out, {rows, top_k}, 5 * rows), ids,
           part(out, {3, rows}, 2 * rows)};
 }
@@ -472,17 +493,15 @@ at::Tensor token_logprobs_backward(const at::Tensor& logits, const at::Tensor& t
   TORCH_CHECK(dlogprob.dim() == 1 && dlogprob.numel() == rows, "dlogprob must hold one value a row");
   TORCH_CHECK(!dentropy || (dentropy->dim() == 1 && dentropy->numel() == rows), "dentropy must hold one value a row");
   at::Tensor to = out ? *out : rows_like(logits);
-  if (rows) {
-    c10::optional<at::Tensor> de;
-    if (dentropy) de = dentropy->contiguous();
-    score_bwd(logits, targets.contiguous(), start, vocab_total, state, dlogprob.contiguous(), de, to);
-  }
+  c10::optional<at::Tensor> de;
+  if (dentropy) de = dentropy->contiguous();
+  score_bwd(logits, targets.contiguous(), start, vocab_total, state, dlogprob.contiguous(), de, to);
   return to;
 }
 at::Tensor pack(const at::Tensor& x) {
   need_matrix(x, "x");
   at::Tensor data = fresh(x, {x.size(0), k::act_pack_row_bytes(x.size(1))}, at::kByte);
-  if (x.size(0)) act_pack(x, data);
+  act_pack(x, data);
   return data;
 }
 Tensors unpack(const at::Tensor& data, int64_t cols, bool fp32, bool gelu) {
@@ -491,7 +510,7 @@ Tensors unpack(const at::Tensor& data, int64_t cols, bool fp32, bool gelu) {
   at::Tensor out = fresh(data, {data.size(0), cols}, type);
   c10::optional<at::Tensor> act;
   if (gelu) act = fresh(data, {data.size(0), cols}, type);
-  if (out.numel()) act_unpack(data, out, act);
+  act_unpack(data, out, act);
   return {out, act};
 }
 Tensors block_join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tensor& pw, const at::Tensor& pb,
@@ -502,19 +521,15 @@ Tensors block_join_fwd(const at::Tensor& x, const at::Tensor& y, const at::Tenso
   at::Tensor u = rows_like(x);
   at::Tensor h = out ? *out : rows_like(x);
   at::Tensor stats = fresh(x, {4, x.size(0)}, at::kFloat);
-  if (x.size(0)) join_fwd(x, y, pw, pb, gate, w, b, u, h, stats, alpha, eps);
+  join_fwd(x, y, pw, pb, gate, w, b, u, h, stats, alpha, eps);
   return {u, h, stats};
 }
 struct Spare {  // gradients of the parameters, and a workspace that is large enough
   at::Tensor grads, workspace;
   Spare(const at::Tensor& dh, bool branch, const c10::optional<at::Tensor>& given) {
     const int64_t rows = dh.size(0), cols = dh.size(1);
-    TORCH_CHECK(cols > 0 && cols <= k::join_max_cols(), "the hidden size is out of range");
+    need_width(cols);
     grads = fresh(dh, {branch ? 5 : 2, cols}, dh.scalar_type());
-    if (!rows) {
-      grads.zero_();
-      return;
-    }
     const int64_t size = join_bwd_workspace(rows, cols, branch);
     workspace = given && given->numel() >= size ? *given : fresh(dh, {size}, at::kFloat);
   }
@@ -534,11 +549,9 @@ Tensors block_join_bwd(const at::Tensor& dh, const c10::optional<at::Tensor>& du
   at::Tensor dx = rows_like(dh);
   c10::optional<at::Tensor> dy = out ? *out : rows_like(dh), h;
   if (b) h = rows_like(dh);
-  if (rows) {
-    const float* s = stats.data_ptr<float>();
-    run_join_bwd(dh, du, u, y, RowStats{s + 2 * rows, s + 3 * rows, s, s + rows}, pw, pb, gate, w, b, dx, dy, h,
-                 spare.grads, spare.workspace, alpha);
-  }
+  const float* s = stats.data_ptr<float>();
+  run_join_bwd(dh, du, u, y, RowStats{s + 2 * rows, s + 3 * rows, s, s + rows}, pw, pb, gate, w, b, dx, dy, h,
+               spare.grads, spare.workspace, alpha);
   const int64_t cols = dh.size(1);
   auto grad = [&](int i) { return part(spare.grads, {cols}, i * cols); };
   return {dx, dy, grad(2), grad(3), grad(4), grad(0), grad(1), h};
@@ -557,9 +570,8 @@ Tensors layer_norm_bwd_packed(const at::Tensor& dy, const c10::optional<at::Tens
   at::Tensor dx = out ? *out : rows_like(dy);
   c10::optional<at::Tensor> y, none;
   if (b) y = rows_like(dy);
-  if (dy.size(0))
-    run_join_bwd(dy, dres, x, none, RowStats{mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr}, none,
-                 none, none, w, b, dx, none, y, spare.grads, spare.workspace, 1.0);
+  run_join_bwd(dy, dres, x, none, RowStats{mean.data_ptr<float>(), rstd.data_ptr<float>(), nullptr, nullptr}, none,
+               none, none, w, b, dx, none, y, spare.grads, spare.workspace, 1.0);
   const int64_t cols = dy.size(1);
   return {dx, part(spare.grads, {cols}, 0), part(spare.grads, {cols}, cols), y};
 }
