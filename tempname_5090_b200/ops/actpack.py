@@ -105,6 +105,7 @@ def _pack_cpu(x):
     finite = torch.where(groups.isfinite(), groups.abs(), torch.zeros(()))
     fraction, exponent = torch.frexp(finite.amax(2))
     exponent = torch.where(fraction > 0.875, exponent - 8, exponent - 9).clamp(min=-126)
+    exponent = torch.where(fraction > 0, exponent, -126)  # zero has no exponent of its own
     scaled = torch.ldexp(groups, -exponent[:, :, None])
     top = torch.where(exponent == 120, 240.0, 448.0)[:, :, None]
     scaled = torch.where(scaled.isfinite(), torch.minimum(scaled.abs(), top).copysign(scaled), torch.full((), float("nan")))
