@@ -137,6 +137,12 @@ def _check_stats(like, shape, **stats):
             raise ValueError(f"{name} must be contiguous FP32 {tuple(shape)} on {like.device}")
 
 
+def _check_workspace(like, workspace):
+    if workspace is not None and (workspace.dtype != torch.float32 or workspace.device != like.device
+                                  or not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be contiguous FP32 on {like.device}")
+
+
 def _check_first(name, t):
     if t.dim() != 2 or t.dtype not in JOIN_DTYPES:
         raise ValueError(f"{name} must be a BF16 or FP32 matrix")
@@ -242,6 +248,7 @@ def block_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pr
                                          residual_scale)
         except (RuntimeError, TypeError):
             _check_join_bwd(dh, dx_out, x_out, y, stats, post_weight, post_bias, gate, pre_weight, pre_bias, out)
+            _check_workspace(dh, workspace)
             raise
         count_launch(2)
         return JoinGrads(*grads)
@@ -303,6 +310,7 @@ def layer_norm_bwd_packed(dy, x, weight, mean, rstd, dres=None, bias=None, works
             dx, dw, db, y = lib().layer_norm_bwd_packed(dy, dres, x.data, mean, rstd, weight, bias, out, workspace)
         except (RuntimeError, TypeError):
             _check_packed_norm(dy, x, weight, mean, rstd, dres, bias, out)
+            _check_workspace(dy, workspace)
             raise
         count_launch(2)
         return dx, dw, db, y
