@@ -598,7 +598,6 @@ void register_kernels(pybind11::module& m) {
   m.def("ce_bwd", &ce_bwd, nogil());
   m.def("score_fwd", &score_fwd, nogil());
   m.def("score_merge", &score_merge, nogil());
-  m.def("score_bwd", &score_bwd, nogil());
   m.def("token_logprobs", &token_logprobs, nogil());
   m.def("token_logprobs_backward", &token_logprobs_backward, nogil());
   m.def("pack", &pack, nogil());
@@ -606,13 +605,9 @@ void register_kernels(pybind11::module& m) {
   m.def("block_join_fwd", &block_join_fwd, nogil());
   m.def("block_join_bwd", &block_join_bwd, nogil());
   m.def("layer_norm_bwd_packed", &layer_norm_bwd_packed, nogil());
-  m.def("act_pack_row_bytes", &k::act_pack_row_bytes);
   m.def("act_pack", &act_pack, nogil());
   m.def("act_unpack", &act_unpack, nogil());
-  m.def("join_fwd", &join_fwd, nogil());
   m.def("join_bwd", &join_bwd, nogil());
-  m.def("join_bwd_workspace", &join_bwd_workspace, nogil());
-  m.def("join_max_cols", &k::join_max_cols);
   m.def("grad_sqsum_parts", &grad_sqsum_parts, nogil());
   m.def("grad_sqsum", &grad_sqsum, nogil());
   m.def("adamw_step", &adamw_step, nogil());

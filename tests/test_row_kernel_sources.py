@@ -214,3 +214,12 @@ def test_limits_of_the_fast_sums():
     bf16_floor = int(re.search(r"floor\(\) \{ return 0x([0-9a-f]{4})\1u; \}  // -kFloor", SCORE)[1], 16)
     bits = torch.tensor([bf16_floor - 0x10000], dtype=torch.int16)
     assert bits.view(torch.bfloat16).item() == -floor
+
+
+def test_native_entries_have_callers():
+    """No entry of the row operators that neither the package nor a test calls."""
+    names = re.findall(r'm\.def\("(\w+)"', BIND)
+    names = names[names.index("ce_bwd") + 1:names.index("grad_sqsum_parts")]
+    root = KERNELS.parents[1]
+    text = "".join(p.read_text() for folder in ("tempname_5090_b200", "tests") for p in (root / folder).rglob("*.py"))
+    assert "token_logprobs" in names and [n for n in names if f"lib().{n}(" not in text] == []
