@@ -13,9 +13,10 @@
 //   unpack_gelu   packed rows -> (x, GeLU(x)) in one pass, the two operands that
 //                 the backward pass of an MLP needs from its pre-activation
 //
-// B200, 8192 x 16384 BF16: pack 66 us (6.1 TB/s), unpack_gelu 126 us (5.3 TB/s, of which
-// four fifths are writes: a plain fill reaches 3.8 TB/s on this GPU); both are bound by
-// memory, unpack_gelu also by its table (shared-memory pipe 71 % busy).
+// B200, 8192 x 16384 BF16, inputs in no cache: pack 67 us (6.0 TB/s), unpack 75 us
+// (5.4 TB/s), unpack_gelu 124 us (5.4 TB/s); bound by memory, unpack_gelu also by its
+// table (shared-memory pipe 71 % busy).  8192 x 4095, value by value: 32, 33 and 63 us
+// (2.1, 2.1 and 2.7 TB/s).
 #include "kernels_api.h"
 #include "rowvec.cuh"
 

@@ -28,12 +28,15 @@
 // row, and threads read single values at the row's offset, columns a CTA's width
 // apart: one barrier more a row.
 //
-// B200, 8192 x 4096 BF16: forward 48 us (5.6 TB/s), gradient 71 us and 6 us for the
-// column sums (5.3 TB/s), LayerNorm's gradient from 8 bits 63 us (4.8 TB/s).  What
-// bounds them is the time that a row's reductions and its few warps take (issue slots
-// 40-55 %, shared-memory pipe 48-62 % busy); more rows at once would need registers
-// (the column sums) or shared memory that an SM has not.  4095 columns, one by one:
-// 96 and 130 us.
+// B200, 8192 x 4096 BF16, inputs in no cache: forward 48 us (5.6 TB/s), gradient 70 us
+// and 9 us for the column sums (5.1 TB/s), from packed rows with h again 113 and 9 us
+// (3.3 TB/s); LayerNorm's gradient from packed rows 50 and 5 us, with its output again
+// 64 and 5 us (4.4 TB/s).  What bounds them is the time that a row's reductions and its
+// few warps take (issue slots 40-55 %, shared-memory pipe 48-62 % busy); more rows at
+// once would need registers (the column sums) or shared memory that an SM has not.
+// 4095 columns, one by one: 96 us forward, 124 and 8 us gradient.  Widths between powers
+// of two have threads for the next one and check bounds: 8192 x 5120 takes 81 us forward
+// (floor 51) and 138 and 8 us gradient (floor 77).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -838,6 +841,7 @@ int fwd_pick(const JoinFwd& p, bool vec, cudaStream_t s) {
 // The gradient's CTAs: as many as fit, but some rows each where that leaves every SM one:
 // every CTA's column sums are written and read once. 777 x 2048: four rows and two cost the
 // same; odd widths, whose rows take longer, 20 us with four and 16 with two at 777 x 2050.
+// No other size was compared.
 template <typename T, int NT, int NV, int FORM, bool BRANCH, bool PACKED>
 int bwd_launch(const JoinBwd& p, JoinFinish f, cudaStream_t s) {
   // Two rows of the widest FP32 tensors are more than an SM holds.

@@ -6,7 +6,7 @@
 //   log p_t = z_t - m - ln s          H = ln s - u / s
 //   d z_j = a ([j = t] - p_j) - b p_j (ln p_j + H)      a = d log p_t, b = d H
 //
-// Forward: a cluster of 1 to 8 CTAs per row, each thread with running (m, s, u)
+// Forward: a cluster of 1, 2 or 4 CTAs per row, each thread with running (m, s, u)
 // in FP32 over 16-byte vectors; a logit of -inf adds nothing.  The alternatives
 // need no sort of the row: the k-th largest of the threads' maxima bounds the k-th
 // largest logit from below, and only the threads that reach it can hold one, so a
@@ -17,12 +17,12 @@
 // Ranks of a vocabulary-parallel group exchange one record a row (m, s, u, z_t
 // and their own alternatives) and merge them in rank order.
 //
-// B200, 8192 BF16 rows of 50304: 128 us without alternatives (6.4 TB/s, the copy's
-// rate; the exponentials keep the special-function units 71-76 % busy, which is what
-// bounds it next), 149 us with 8 and 179 us with 32 of them (the second look and the
-// sorts, between barriers).  Inputs that are not in any cache add 11 us.  Splitting a
-// row over more threads or CTAs costs more than it gives where rows are many.
-// Gradient of 2048 rows: 64 us (6.5 TB/s).
+// B200, 8192 BF16 rows of 50304 in no cache: 140 us without alternatives (5.9 TB/s; the
+// exponentials keep the special-function units 71-76 % busy, which is what bounds it
+// next), 160 us with 8 and 192 us with 32 of them (the second look and the sorts,
+// between barriers); 11 us less where the call before had the same inputs.  8192 rows of
+// 6288: 28, 42 and 73 us, of 1000 with 8 alternatives 26 us: a row's fixed chain of
+// steps.  Gradient of 2048 rows of 50304: 70 us (5.9 TB/s).
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -797,8 +797,10 @@ int score_threads(const void* logits, int64_t ld, unsigned vocab, const int64_t*
 template <typename T>
 int score_typed(const void* logits, int64_t ld, unsigned vocab, const int64_t* targets, int64_t start,
                 int64_t vocab_total, const Out& o, cudaStream_t s) {
-  // A row is split over a cluster while the rows alone leave SMs idle (1 row of 50304: 9.5 us
-  // on four CTAs, 11.6 us on one; with more rows than SMs the split only costs).
+  // A row is split over a cluster while the rows alone leave SMs idle: 1 row of 50304 takes
+  // 9.5 us on four CTAs and 11.6 us on one, 8192 rows 226 us on two each and 150 us on one.
+  // In between no split was compared; one CTA each takes 12.1 us for 128 rows and 20.0 us
+  // for 592, with 8 alternatives.
   unsigned C = 1;
   while (C < 4 && int64_t(o.rows) * C * 2 <= 148 && vocab / (2 * C) >= 4096) C *= 2;
   // Threads of a row's CTA: what a row costs beside its loads (joining the threads' sums
@@ -834,7 +836,7 @@ int score_bwd_typed(const void* logits, int64_t ld, int rows, unsigned vocab, co
   return int(cudaGetLastError());
 }
 bool sizes_fit(int64_t rows, int64_t vocab, int64_t vocab_total) {
-  // Ids travel as 32-bit integers; a launch has rows * 8 CTAs at most.
+  // Ids travel as 32-bit integers; a launch has a CTA for each row, or 148 in clusters.
   return rows > 0 && vocab > 0 && rows <= 0x7fffffff / 8 && vocab_total <= 0x7fffffff;
 }
 }  // namespace

@@ -470,9 +470,10 @@ class GPT:
         """Forward + backward of one micro-batch; gradients of `loss * loss_scale`
         are written into `self.store.grad`.  Returns the (unscaled) mean loss.
 
-        The loss is the mean cross-entropy; with `weights` (FP32, one a position) or an
-        `entropy_bonus` it is -mean(weight * log p(target) + entropy_bonus * entropy) over
-        the positions, of which those with a negative target count as zero."""
+        The loss is the mean cross-entropy, whose targets all lie in the vocabulary; with
+        `weights` (FP32, one a position) or an `entropy_bonus` it is
+        -mean(weight * log p(target) + entropy_bonus * entropy) over the positions, of
+        which those with a negative target count as zero whatever their weight."""
         if weights is None and entropy_bonus == 0.0:
             loss, tape = self._forward(tokens, targets, keep=True, loss_scale=1.0)
             self._backward(tape, loss_scale)
