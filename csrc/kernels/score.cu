@@ -707,10 +707,12 @@ __global__ void __launch_bounds__(kThreads) score_bwd_kernel(const T* logits, in
   float a = target >= 0 ? dlogprob[row] : 0.f;
   const float b = dentropy ? dentropy[row] : 0.f;
   if (target >= vocab_total || m != m) a = __int_as_float(0x7fffffff);
-  const bool empty = m == -INFINITY;
+  // Without a gradient: a row that the mask emptied, and one that is not scored, whatever
+  // its logits hold (`gradient` lifts NaN to kLowest, so that zero factors give zeros).
+  const bool empty = m == -INFINITY || (target < 0 && b == 0.f);
   const int64_t local = target - start;
   const unsigned at = local >= 0 && local < vocab ? unsigned(local) : 0xffffffffu;
-  // -p (a + b (l + H)) as p (c0 + c1 l), l = ln p; nothing in a row that the mask emptied.
+  // -p (a + b (l + H)) as p (c0 + c1 l), l = ln p.
   const float c1 = empty ? 0.f : -b, c0 = empty ? 0.f : -a - b * H;
   auto gradient = [&](float z, unsigned i) {
     const float l = fmaxf((z - m) - ln_s, kLowest);

@@ -127,10 +127,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, 
                    world: int = 1):
     """Return (TokenScores, ScoreState) of logits [M, V/world] (this rank's shard).
 
-    A negative target is not scored (log probability 0, which passes no gradient on;
-    the entropy is the row's all the same); one at or above the vocabulary's end
-    gives NaN.  A logit of -inf is a token that cannot
-    occur; a row of nothing else has log probability -inf, entropy 0 and no
+    A negative target is not scored (log probability 0, which passes no gradient on
+    whatever the row holds; the entropy is the row's all the same); one at or above
+    the vocabulary's end gives NaN.  A logit of -inf is a token that cannot occur; a
+    row of nothing else has log probability -inf, entropy 0 and no
     gradient.  A NaN or +inf makes its row's numbers NaN.  `top_k` is at most 32
     and at most the shard's vocabulary.
     """
@@ -239,10 +239,10 @@ def _score_gradient_cpu(logits, targets, state, dlogprob, dentropy, out):
     M, V = logits.shape
     out = torch.empty((M, V), dtype=logits.dtype) if out is None else out
     m, log_s, entropy = state.stats
-    empty = m == -torch.inf
+    b = torch.zeros(M) if dentropy is None else dentropy
+    empty = (m == -torch.inf) | ((targets < 0) & (b == 0))  # no gradient, whatever the logits hold
     a = torch.where(targets >= 0, dlogprob, torch.zeros(()))
     a = torch.where((targets >= state.vocab) | m.isnan(), torch.full((), float("nan")), a)
-    b = torch.zeros(M) if dentropy is None else dentropy
     logp = ((logits.float() - torch.where(empty, torch.zeros(()), m)[:, None]) - log_s[:, None]).clamp(min=-200.0)
     g = -logp.exp() * (a[:, None] + b[:, None] * (logp + entropy[:, None]))
     local = targets - state.start
